@@ -13,6 +13,8 @@ void register_optim(pybind11::module_& m);
 void register_comm(pybind11::module_& m);
 void register_ep(pybind11::module_& m);
 void register_dp(pybind11::module_& m);
+void register_paged(pybind11::module_& m);
+void register_beam(pybind11::module_& m);
 }  // namespace dsv3
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -27,4 +29,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   dsv3::register_comm(m);
   dsv3::register_ep(m);
   dsv3::register_dp(m);
+  dsv3::register_paged(m);
+  dsv3::register_beam(m);
 }

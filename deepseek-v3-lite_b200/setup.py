@@ -16,7 +16,7 @@ os.environ.setdefault("MAX_JOBS", str(min(8, os.cpu_count() or 1)))
 
 SOURCES = ["csrc/bindings.cpp", "csrc/status.cu", "csrc/gemm.cu", "csrc/elementwise.cu", "csrc/moe.cu",
            "csrc/attention.cu", "csrc/optim.cu", "csrc/comm.cu", "csrc/ep.cu", "csrc/dp.cu",
-           "csrc/latent_decode_noalloc.cu"]
+           "csrc/latent_decode_noalloc.cu", "csrc/paged.cu", "csrc/beam.cu"]
 
 NVCC = ["-O3", "-lineinfo", "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a",
         "--expt-relaxed-constexpr", "-Xptxas", "-v" if os.environ.get("DSV3_PTXAS_VERBOSE") else "-O3",
