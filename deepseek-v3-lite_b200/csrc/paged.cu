@@ -24,6 +24,7 @@
 
 #include "common.cuh"
 #include "status.h"
+#include "tma_host.h"
 
 namespace dsv3 {
 
@@ -93,61 +94,7 @@ __global__ void __launch_bounds__(128) latent_append_kernel(const T* __restrict_
 }
 
 // ---------------------------------------------------------------- attention
-// out[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) k_j[:R] over the cached
-// rows j at or before the token's position.  One warp per (token, head) with a
-// running maximum and sum.
-constexpr int kMaxPerLane = 18;  // D <= 576
-
-__global__ void __launch_bounds__(128) paged_attention_kernel(const bf16* __restrict__ q, int total, int H, int R,
-                                                              int D, Ragged rg, const bf16* __restrict__ pages,
-                                                              long ld_page, long ld_row, float scale,
-                                                              bf16* __restrict__ out, unsigned int* status) {
-  const int item = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (item >= total * H) return;
-  const int t = item / H;
-  const int b = ragged_seq(rg, t, lane);
-  int keys = 0;
-  if (b < rg.B) {
-    const int len = min(rg.lens[b], rg.cols * rg.page);
-    keys = min(rg.lens[b] - rg.cu[b + 1] + t + 1, len);
-    if (len < rg.lens[b] && lane == 0) record_error(status, DSV3_ERR_BOUNDS);
-  } else if (lane == 0) {
-    record_error(status, DSV3_ERR_BOUNDS);
-  }
-  float qv[kMaxPerLane], acc[kMaxPerLane], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < kMaxPerLane; ++i) {
-    acc[i] = 0.f;
-    qv[i] = lane + 32 * i < D ? __bfloat162float(q[(size_t)item * D + lane + 32 * i]) : 0.f;
-  }
-  for (int j = 0; j < keys; ++j) {
-    const int pg = rg.table[b * rg.ldt + j / rg.page];
-    if (pg < 0 || pg >= rg.pool) {
-      if (lane == 0) record_error(status, DSV3_ERR_BOUNDS);
-      continue;
-    }
-    const bf16* kr = pages + (size_t)pg * ld_page + (size_t)(j % rg.page) * ld_row;
-    float kv[kMaxPerLane], s = 0.f;
-#pragma unroll
-    for (int i = 0; i < kMaxPerLane; ++i) {
-      kv[i] = lane + 32 * i < D ? __bfloat162float(kr[lane + 32 * i]) : 0.f;
-      s += qv[i] * kv[i];
-    }
-    s = warp_sum(s) * scale;
-    const float nm = fmaxf(m, s);
-    if (nm == -INFINITY) continue;
-    const float c = expf(m - nm), p = expf(s - nm);
-    l = l * c + p;
-#pragma unroll
-    for (int i = 0; i < kMaxPerLane; ++i) acc[i] = acc[i] * c + p * kv[i];
-    m = nm;
-  }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-#pragma unroll
-  for (int i = 0; i < kMaxPerLane; ++i)
-    if (lane + 32 * i < R) out[(size_t)item * R + lane + 32 * i] = __float2bfloat16(acc[i] * inv);
-}
+#include "paged_attention_tc.cuh"
 
 // --------------------------------------------------------------- host side
 Ragged check_ragged(const char* op, const at::Tensor& ref, const at::Tensor& pages, const at::Tensor& table,
@@ -170,6 +117,7 @@ Ragged check_ragged(const char* op, const at::Tensor& ref, const at::Tensor& pag
   TORCH_CHECK(pages.stride(0) % 8 == 0 && pages.stride(1) % 8 == 0 &&
                   reinterpret_cast<uintptr_t>(pages.data_ptr()) % 16 == 0,
               op, ": page rows must be 16-byte aligned");
+  TORCH_CHECK(pages.size(0) >= 1 && table.size(1) >= 1, op, ": an empty pool or table");
   TORCH_CHECK(pages.size(0) * page < (1ll << 31) && table.size(1) * page < (1ll << 31), op,
               ": the pool and a sequence hold fewer than 2^31 rows");
   Ragged r;
@@ -234,16 +182,49 @@ at::Tensor paged_latent_attention(const at::Tensor& q, const at::Tensor& pages, 
   TORCH_CHECK(R % 8 == 0 && R >= 8 && R <= 512 && D % 8 == 0 && D > R && D - R <= 64, op,
               ": the latent rank must be a multiple of 8 up to 512 and the rotary width one up to 64, got ",
               std::to_string(R), " and ", std::to_string(D - R));
-  TORCH_CHECK(H >= 1 && T * H < (1ll << 31), op, ": T * H must be below 2^31");
+  TORCH_CHECK(H >= 1 && H <= 4096 && T * H < (1ll << 31), op, ": 1 to 4096 heads and T * H below 2^31");
+  TORCH_CHECK(scale > 0, op, ": scale must be positive");
   auto out = at::empty({T, H, R}, q.options());
   if (T == 0) return out;
   TORCH_CHECK(rg.B > 0, op, ": tokens without a sequence");
   const at::cuda::CUDAGuard guard(pages.device());
-  paged_attention_kernel<<<(int)((T * H + 3) / 4), 128, 0, at::cuda::getCurrentCUDAStream()>>>(
-      reinterpret_cast<const bf16*>(q.data_ptr()), (int)T, (int)H, (int)R, (int)D, rg,
-      reinterpret_cast<const bf16*>(pages.data_ptr()), pages.stride(0), pages.stride(1), (float)scale,
-      reinterpret_cast<bf16*>(out.data_ptr()), status_ptr());
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  // Row tile: 16 and 32 where a sequence has that many rows on average (a
+  // decode step), else 64, or 128 where the output columns of a 128-row tile
+  // fit in TMEM and the sequences fill it.
+  const int64_t rows = (T * H + rg.B - 1) / rg.B;
+  const int N = rows <= 16 ? 16 : rows <= 32 && T == rg.B ? 32 : rows <= 64 || R > 256 ? 64 : 128;
+  PagedPlan pl;
+  TORCH_CHECK(paged_plan(N, (int)R, (int)D, pl), op, ": no shared-memory plan");
+  auto work = at::empty({sms * (2 * N * (R + 2) + 4)}, q.options().dtype(at::kFloat));
+  int4* rec = reinterpret_cast<int4*>(work.data_ptr<float>());
+  float2* ml = reinterpret_cast<float2*>(rec + sms);
+  float* part = reinterpret_cast<float*>(ml + 2 * (int64_t)sms * N);
+  const uint64_t qd[2] = {(uint64_t)D, (uint64_t)(T * H)}, qs[1] = {(uint64_t)D * 2};
+  const uint32_t qb[2] = {64, (uint32_t)N};
+  const CUtensorMap tm_q = make_map(q.data_ptr(), 2, qd, qs, qb);
+  const uint64_t kd[3] = {(uint64_t)D, (uint64_t)rg.page, (uint64_t)rg.pool};
+  const uint64_t ks[2] = {(uint64_t)pages.stride(1) * 2, (uint64_t)pages.stride(0) * 2};
+  const uint32_t kb[3] = {64, (uint32_t)std::min(rg.page, 128), 1};
+  const CUtensorMap tm_kv = make_map(pages.data_ptr(), 3, kd, ks, kb);
+  auto st = at::cuda::getCurrentCUDAStream();
+  bf16* o = reinterpret_cast<bf16*>(out.data_ptr());
+#define DSV3_PAGED(N_)                                                                                           \
+  do {                                                                                                           \
+    C10_CUDA_CHECK(cudaFuncSetAttribute(paged_attention_tc_kernel<N_>,                                           \
+                                        cudaFuncAttributeMaxDynamicSharedMemorySize, pl.smem));                  \
+    paged_attention_tc_kernel<N_><<<sms, kPaThreads, pl.smem, st>>>(                                             \
+        tm_q, tm_kv, pl, rg, (int)T, (int)H, (int)R, (int)D, (float)(scale * 1.4426950408889634), 1, o, part, ml, \
+        rec, status_ptr());                                                                                      \
+    C10_CUDA_KERNEL_LAUNCH_CHECK();                                                                              \
+    paged_merge_kernel<N_><<<dim3(sms, N_), 128, 0, st>>>(part, ml, rec, (int)R, o);                             \
+    C10_CUDA_KERNEL_LAUNCH_CHECK();                                                                              \
+  } while (0)
+  if (N == 16) DSV3_PAGED(16);
+  else if (N == 32) DSV3_PAGED(32);
+  else if (N == 64) DSV3_PAGED(64);
+  else DSV3_PAGED(128);
+#undef DSV3_PAGED
   return out;
 }
 
