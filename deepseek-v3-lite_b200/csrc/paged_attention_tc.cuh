@@ -63,7 +63,7 @@ inline bool paged_plan(int N, int R, int D, PagedPlan& p) {
   p.nch = (D + 63) / 64;
   p.tail = D > 128 * p.LP ? 1 : 0;
   const int limit = 232448;
-  const int q = p.nch * N * 128, P = (N + 63) / 64 * kPaChunk, misc = 8 * N + 1024 + 512;
+  const int q = p.nch * N * 128, P = (N + 63) / 64 * kPaChunk, misc = 12 * N + 1024 + 512;
   for (int mode = 0; mode < 3; ++mode) {     // two tail slots, one, one shared with P
     p.tails = p.tail ? (mode == 0 ? 2 : 1) : 0;
     p.alias = p.tail && mode == 2;
@@ -88,23 +88,25 @@ inline bool paged_plan(int N, int R, int D, PagedPlan& p) {
 }
 
 // sum_{i=0}^{n-1} floor((a i + b) / m) for a, b >= 0 (Euclid-like reduction, a
-// few steps).
-__device__ __forceinline__ long long floor_sum(long long n, long long m, long long a, long long b) {
+// few steps).  T is 32 bits wide where a n + b fits: its division is several
+// times cheaper.
+template <typename T>
+__device__ __forceinline__ long long floor_sum(T n, T m, T a, T b) {
   long long ans = 0;
   while (n > 0) {
     if (a >= m) {
-      ans += (n - 1) * n / 2 * (a / m);
+      ans += (long long)(n - 1) * n / 2 * (a / m);
       a %= m;
     }
     if (b >= m) {
-      ans += n * (b / m);
+      ans += (long long)n * (b / m);
       b %= m;
     }
-    const long long y = a * n + b;
+    const T y = a * n + b;
     if (y < m) break;
     n = y / m;
     b = y % m;
-    const long long t = m;
+    const T t = m;
     m = a;
     a = t;
   }
@@ -150,11 +152,13 @@ __device__ __forceinline__ long long paged_tiles_before(const PagedSeq& s, int k
   }
   // row tile i ends at row x = (i + 1) N - 1, at position p = len - n + x / H:
   // p / 128 + 1 = ((len - n) H + x) / (128 H) + 1 tiles, one where p < 0
-  const long long m = 128ll * H, c = (long long)(s.len - s.n) * H + N - 1;
+  const long long c = (long long)(s.len - s.n) * H + N - 1;
   int first = 0;
   if (c < 0) first = (int)min((long long)full, (-c + N - 1) / N);
-  ans += full + floor_sum(full - first, m, N, c + (long long)first * N);
-  return ans;
+  const long long b = c + (long long)first * N;
+  if (b + (long long)full * N < (1ll << 31))
+    return ans + full + floor_sum<uint32_t>(full - first, 128u * H, N, (uint32_t)b);
+  return ans + full + floor_sum<long long>(full - first, 128ll * H, N, b);
 }
 
 // A CTA's share as a walk over items: (sequence, row tile, key tiles t0 .. t1).
@@ -244,31 +248,36 @@ struct PagedStart {
   long long count;            // key tiles in the share
   long long share;
   long long first;            // flat index of its first key tile
+  long long local;            // its index within sequence b
   int b, rt, tile;
 };
 
 template <int N>
 __device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, int min_share, PagedStart* out,
-                                           long long* warp_sum, unsigned int* status) {
+                                           long long* scan, unsigned int* status) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int NW = kPaThreads / 32;
-  // round 0 adds up all sequences; round 1 finds the one that holds the share's first tile
-  long long W = 0, target = 0;
+  // round 0 adds up all sequences; round 1 finds the one that holds the share's
+  // first tile (a batch of up to kPaThreads sequences is still in registers)
+  long long target = 0, t = 0;
+  PagedSeq s;
+  s.tiles = 0;
   for (int round = 0; round < 2; ++round) {
     long long base = 0;
     for (int b0 = 0; b0 < r.B; b0 += kPaThreads) {
       const int b = b0 + tid;
-      PagedSeq s;
-      s.tiles = 0;
-      long long t = 0;
-      if (b < r.B) {
-        s = paged_seq<N>(r, b, H, total);
-        t = paged_tiles_before<N>(s, s.tiles, H);
-        if (round == 0 && blockIdx.x == 0) {
-          const bool bad = __ldg(r.lens + b) > r.cols * r.page || __ldg(r.cu + b + 1) > total ||
-                           __ldg(r.cu + b + 1) < __ldg(r.cu + b) || (b == 0 && __ldg(r.cu) != 0) ||
-                           (b == r.B - 1 && __ldg(r.cu + b + 1) != total);
-          if (bad) record_error(status, DSV3_ERR_BOUNDS);
+      if (round == 0 || r.B > kPaThreads) {
+        s.tiles = 0;
+        t = 0;
+        if (b < r.B) {
+          s = paged_seq<N>(r, b, H, total);
+          t = paged_tiles_before<N>(s, s.tiles, H);
+          if (round == 0 && blockIdx.x == 0) {
+            const int c0 = __ldg(r.cu + b), c1 = __ldg(r.cu + b + 1);
+            if (__ldg(r.lens + b) > r.cols * r.page || c1 > total || c1 < c0 || (b == 0 && c0 != 0) ||
+                (b == r.B - 1 && c1 != total))
+              record_error(status, DSV3_ERR_BOUNDS);
+          }
         }
       }
       long long inc = t;
@@ -277,45 +286,130 @@ __device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, in
         const long long v = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += v;
       }
-      if (lane == 31) warp_sum[warp] = inc;
+      if (lane == 31) scan[warp] = inc;
       __syncthreads();
       long long before = base, all = base;
+#pragma unroll
       for (int w = 0; w < NW; ++w) {
-        if (w < warp) before += warp_sum[w];
-        all += warp_sum[w];
+        const long long v = scan[w];
+        if (w < warp) before += v;
+        all += v;
       }
-      const long long lo = before + inc - t, hi = before + inc;
-      if (round == 1 && t > 0 && lo <= target && target < hi) {
-        // last row tile that starts at or before the target
-        int a = 0, z = s.tiles - 1;
-        while (a < z) {
-          const int mid = (a + z + 1) >> 1;
-          if (lo + paged_tiles_before<N>(s, mid, H) <= target) a = mid;
-          else z = mid - 1;
-        }
+      if (round == 1 && t > 0 && before + inc - t <= target && target < before + inc) {
         out->b = b;
-        out->rt = a;
-        out->tile = (int)(target - lo - paged_tiles_before<N>(s, a, H));
+        out->local = target - (before + inc - t);
       }
       base = all;
       __syncthreads();
     }
     if (round == 0) {
-      W = base;
-      long long share = (W + gridDim.x - 1) / gridDim.x;
+      long long share = (base + gridDim.x - 1) / gridDim.x;
       if (share < min_share) share = min_share;
       target = share * blockIdx.x;
       if (tid == 0) {
         out->share = share;
         out->first = target;
-        out->count = min(share, W - target);
+        out->count = min(share, base - target);
         out->b = out->rt = out->tile = 0;
+        out->local = 0;
       }
-      if (target >= W) break;
+      if (target >= base) break;
     }
   }
   __syncthreads();
+  if (out->count > 0) {   // the row tile of that sequence: every thread tries one candidate
+    const long long local = out->local;
+    s = paged_seq<N>(r, out->b, H, total);
+    int lo = 0, hi = s.tiles;                    // the answer lies in [lo, hi)
+    while (hi > lo) {
+      const int step = (hi - lo + kPaThreads - 1) / kPaThreads, k = lo + tid * step;
+      const int k1 = min(k + step, hi);
+      if (k < hi) {
+        const long long at = paged_tiles_before<N>(s, k, H);
+        if (at <= local && (k1 == s.tiles || local < paged_tiles_before<N>(s, k1, H))) {
+          out->rt = k;
+          out->tile = (int)(local - at);
+        }
+      }
+      __syncthreads();
+      lo = out->rt;
+      hi = step > 1 ? min(lo + step, hi) : lo;
+      __syncthreads();
+    }
+  }
 }
+
+// Combines W values per lane over the 32 lanes of a warp, column by column: W
+// / 2 exchanges, then W / 4 ..., since a lane keeps only half of its columns at
+// each step.  Lane i ends with column i * W / 32.
+template <int W, typename Op>
+__device__ __forceinline__ float fold_columns(float (&v)[W], int lane, Op op) {
+  int o = 16;
+#pragma unroll
+  for (int w = W; w > 1; w >>= 1, o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int i = 0; i < w / 2; ++i) {
+      const float send = up ? v[i] : v[i + w / 2], keep = up ? v[i + w / 2] : v[i];
+      v[i] = op(keep, __shfl_xor_sync(0xffffffffu, send, o));
+    }
+  }
+  for (; o > 0; o >>= 1) v[0] = op(v[0], __shfl_xor_sync(0xffffffffu, v[0], o));
+  return v[0];
+}
+
+// One MMA by the lane whose `leader` is set.  The whole warp runs the issuing
+// code with the same values: descriptors then stay in uniform registers, where
+// the instruction wants them (one lane in a divergent branch moved each operand
+// there first and issued an MMA in 90 to 190 cycles).
+__device__ __forceinline__ void umma_lead(uint32_t leader, uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi,
+                                          uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "setp.ne.b32 q, %0, 0;\n\t"
+      "mov.b64 da, {%2, %4};\n\t"
+      "mov.b64 db, {%3, %4};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%1], da, db, %5, p;\n\t}" ::"r"(leader),
+      "r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void commit_lead(uint32_t leader, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %0, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}" ::"r"(leader),
+      "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ uint32_t elect_lead() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r;
+}
+
+// Low words of the shared-memory descriptors (128-byte swizzle, 1024 bytes
+// between groups of eight rows) and the high word that both share.
+constexpr uint32_t kPaDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k(uint32_t addr) { return (addr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t addr) { return (addr >> 4) | ((uint32_t)(kPaChunk >> 4) << 16); }
+
+// Position in a ring of slots.
+struct Ring {
+  int n, slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ explicit Ring(int n_) : n(n_) {}
+  __device__ __forceinline__ void next() {
+    if (++slot >= n) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+};
 
 template <int N>
 __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
@@ -326,7 +420,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
   extern __shared__ __align__(1024) uint8_t smem[];
   float* mref = reinterpret_cast<float*>(smem + pl.off_misc);            // [N]
   int* lim = reinterpret_cast<int*>(mref + N);                           // [N] keys that a row sees
-  float* red = reinterpret_cast<float*>(lim + N);                        // [2][32][4]
+  float* corr = reinterpret_cast<float*>(lim + N);                       // [N] rescaling, 1 / sum, or maximum keys
+  float* red = corr + N;                                                 // [2][32][4]
   uint64_t* pair_full = reinterpret_cast<uint64_t*>(red + 256);
   uint64_t* pair_empty = pair_full + kPaMaxSlots;
   uint64_t* tail_full = pair_empty + kPaMaxSlots;
@@ -343,7 +438,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(scan + kPaThreads / 32);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < pl.slots; ++i) {
       mbar_init(&pair_full[i], 1);
@@ -381,6 +476,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
+    Ring pr(pl.slots), tr(pl.tail ? pl.tails : 1);
     uint32_t pu = 0, tu = 0, items = 0;      // pair uses, tail uses
     bool ok = count > 0;
     for (PagedWalk<N> w(rg, H, total, ok ? count : 0, start->b, start->rt, start->tile); w.ok() && ok; w.next(), ++items) {
@@ -410,8 +506,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
           if (m == pl.LP && !pl.tail) break;
           const bool is_tail = m == pl.LP;
           const int c0 = 2 * m, nc = is_tail ? 1 : min(2, pl.nch - c0);
-          const int slot = is_tail ? tu % pl.tails : pu % pl.slots;
-          const uint32_t ph = (is_tail ? tu / pl.tails : pu / pl.slots) & 1u;
+          const int slot = is_tail ? tr.slot : pr.slot;
+          const uint32_t ph = is_tail ? tr.phase : pr.phase;
           uint64_t* full = is_tail ? &tail_full[slot] : &pair_full[slot];
           uint64_t* empty = is_tail ? &tail_empty[slot] : &pair_empty[slot];
           uint8_t* at = smem + (is_tail ? pl.off_t + slot * kPaChunk : slot * kPaPair);
@@ -423,8 +519,13 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
           if (ok && lane < boxes)
             for (int c = 0; c < nc; ++c) tma_load_3d(at + c * kPaChunk + dst, &tm_kv, full, 64 * (c0 + c), row, pg);
           if (ok) {
-            if (is_tail) ++tu;
-            else ++pu;
+            if (is_tail) {
+              tr.next();
+              ++tu;
+            } else {
+              pr.next();
+              ++pu;
+            }
           }
         }
       }
@@ -440,14 +541,17 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer
-    if (lane == 0 && count > 0) {
+    if (count > 0) {
       constexpr uint32_t I_S = idesc_bf16_f32(128, N, 0, 0);     // S^T = K Q^T
       constexpr uint32_t I_O = idesc_bf16_f32(128, N, 1, 1);     // O^T += V^T P^T, both read MN-major
+      const uint32_t lead = elect_lead();
       PagedWalk<N> ws(rg, H, total, count, start->b, start->rt, start->tile);   // walk of S
       PagedWalk<N> wp(rg, H, total, count, start->b, start->rt, start->tile);   // walk of PV
+      Ring sr(pl.slots), tr(pl.tail ? pl.tails : 1), vr(pl.slots);
       int ts = ws.t0, tp = wp.t0;
-      uint32_t gs = 0, gp = 0, s_items = 0, p_items = 0, tu = 0;
+      uint32_t gs = 0, gp = 0, s_items = 0, p_items = 0;
       bool ok = true, issued = false;
+      const uint32_t p_lo = desc_mn(smem0 + pl.off_p);
       // S^T of the next tile in order
       auto issue_s = [&]() {
         if (ts == ws.t0) {
@@ -455,36 +559,39 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
         }
         const uint32_t d = tmem + (gs & 1u) * N;
         uint32_t acc = 0;
-        for (int m = 0; m <= pl.LP; ++m) {
-          if (m == pl.LP && !pl.tail) break;
+        uint32_t q_lo = desc_k(smem0 + pl.off_q);
+        for (int m = 0; m < pl.LP + pl.tail; ++m) {
           const bool is_tail = m == pl.LP;
-          const uint32_t u = is_tail ? tu : gs * pl.LP + m;
-          const int ring = is_tail ? pl.tails : pl.slots;
-          const int slot = u % ring;
-          if (!mbar_wait_bounded(is_tail ? &tail_full[slot] : &pair_full[slot], (u / ring) & 1u, abort_flag, status,
-                                 DSV3_ERR_WAIT_FULL))
+          const int slot = is_tail ? tr.slot : sr.slot;
+          if (!mbar_wait_bounded(is_tail ? &tail_full[slot] : &pair_full[slot], is_tail ? tr.phase : sr.phase,
+                                 abort_flag, status, DSV3_ERR_WAIT_FULL))
             return false;
           tc_fence_after();
-          const int nc = is_tail ? 1 : min(2, pl.nch - 2 * m);
-          const uint32_t at = smem0 + (is_tail ? pl.off_t + slot * kPaChunk : slot * kPaPair);
-          for (int c = 0; c < nc; ++c) {
-            const int ch = 2 * m + c, ks = min(4, (D - 64 * ch + 15) / 16);
-            for (int kk = 0; kk < ks; ++kk) {
-              umma_bf16(d, smem_desc_sw128(at + c * kPaChunk + kk * 32, 16, 1024),
-                        smem_desc_sw128(smem0 + pl.off_q + ch * N * 128 + kk * 32, 16, 1024), I_S, acc);
-              acc = 1;
-            }
+          uint32_t a_lo = desc_k(smem0 + (is_tail ? pl.off_t + slot * kPaChunk : slot * kPaPair));
+          int left = D - 128 * m;               // columns of this pair that hold data
+          for (int c = 0; c < 2 && left > 0; ++c) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              if (16 * kk < left) {
+                umma_lead(lead, d, a_lo + 2 * kk, q_lo + 2 * kk, kPaDescHi, I_S, acc);
+                acc = 1;
+              }
+            a_lo += kPaChunk >> 4;
+            q_lo += N * 128 >> 4;
+            left -= 64;
           }
           issued = true;
           if (is_tail) {
-            if (!pl.alias) umma_commit(&tail_empty[slot]);
-            ++tu;
+            if (!pl.alias) commit_lead(lead, &tail_empty[slot]);
+            tr.next();
+          } else {
+            sr.next();
           }
         }
-        umma_commit(&s_full[gs & 1u]);
+        commit_lead(lead, &s_full[gs & 1u]);
         ++gs;
         if (++ts >= ws.t1) {
-          umma_commit(q_empty);
+          commit_lead(lead, q_empty);
           ++s_items;
           ws.next();
           ts = ws.t0;
@@ -502,14 +609,15 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
           break;
         tc_fence_after();
         for (int m = 0; m < pl.LP; ++m) {
-          const int slot = (gp * pl.LP + m) % pl.slots;
-          for (int kk = 0; kk < 8; ++kk)
-            umma_bf16(tmem + (2 + m) * N, smem_desc_sw128(smem0 + slot * kPaPair + kk * 2048, kPaChunk, 1024),
-                      smem_desc_sw128(smem0 + pl.off_p + kk * 2048, kPaChunk, 1024), I_O, !first || kk > 0);
-          umma_commit(&pair_empty[slot]);
+          const uint32_t v_lo = desc_mn(smem0 + vr.slot * kPaPair), d = tmem + (2 + m) * N;
+          umma_lead(lead, d, v_lo, p_lo, kPaDescHi, I_O, first ? 0u : 1u);
+#pragma unroll
+          for (int kk = 1; kk < 8; ++kk) umma_lead(lead, d, v_lo + 128 * kk, p_lo + 128 * kk, kPaDescHi, I_O, 1u);
+          commit_lead(lead, &pair_empty[vr.slot]);
+          vr.next();
         }
-        if (pl.alias) umma_commit(&tail_empty[0]);
-        umma_commit(pv_done);
+        if (pl.alias) commit_lead(lead, &tail_empty[0]);
+        commit_lead(lead, pv_done);
         issued = true;
         ++gp;
         if (++tp >= wp.t1) {
@@ -520,9 +628,10 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
         if (!pl.look && ws.ok()) ok = issue_s();
       }
       if (issued) {   // no MMA may still write TMEM when it is freed
-        umma_commit(drain);
+        commit_lead(lead, drain);
         mbar_wait_bounded(drain, 0, nullptr, status, DSV3_ERR_WAIT_TMEM);
       }
+      __syncwarp();
     }
   } else {
     // ---------------------------------------------------- softmax / epilogue
@@ -544,6 +653,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
       if (ht < NC) {
         const int n = col0 + ht;
         mref[n] = kPaUnset;
+        reinterpret_cast<uint32_t*>(corr)[n] = 0u;
         lim[n] = n < nr ? base + (w.rt * N + n) / H + 1 : 0;
       }
       half_sync(half);
@@ -568,83 +678,82 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
             if (pos >= k4.w) sr[c + 3] = 0xff800000u;
           }
         }
-        float over = -INFINITY;
+        // p = 2^(s - m) at the present references; where one is passed by more
+        // than 2^8 the half moves them and computes p again
+        uint32_t pk[NC / 2];
+        for (int attempt = 0;; ++attempt) {
+          float over = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < NC; c += 4) {
-          const float4 m4 = mref4[c / 4];
-          over = fmaxf(over, fmaf(__uint_as_float(sr[c]), scale_log2, -m4.x));
-          over = fmaxf(over, fmaf(__uint_as_float(sr[c + 1]), scale_log2, -m4.y));
-          over = fmaxf(over, fmaf(__uint_as_float(sr[c + 2]), scale_log2, -m4.z));
-          over = fmaxf(over, fmaf(__uint_as_float(sr[c + 3]), scale_log2, -m4.w));
+          for (int c = 0; c < NC; c += 4) {
+            const float4 m4 = mref4[c / 4];
+            const float d0 = fmaf(__uint_as_float(sr[c]), scale_log2, -m4.x);
+            const float d1 = fmaf(__uint_as_float(sr[c + 1]), scale_log2, -m4.y);
+            const float d2 = fmaf(__uint_as_float(sr[c + 2]), scale_log2, -m4.z);
+            const float d3 = fmaf(__uint_as_float(sr[c + 3]), scale_log2, -m4.w);
+            over = fmaxf(fmaxf(over, fmaxf(d0, d1)), fmaxf(d2, d3));
+            pk[c / 2] = pack_bf16x2(ex2_approx(d0), ex2_approx(d1));
+            pk[c / 2 + 1] = pack_bf16x2(ex2_approx(d2), ex2_approx(d3));
+          }
+          if (!half_any(half, over > 8.f) || attempt == 1) break;
+          // column maxima of the tile: S^T is read again in slices, so that this
+          // rare path is a short loop (unrolled over registers it ran from
+          // instruction-cache misses, 14,000 cycles)
+          constexpr int W = NC < 16 ? NC : 16;
+#pragma unroll 1
+          for (int c0 = 0; c0 < NC; c0 += W) {
+            uint32_t u[W];
+            float v[W];
+            tmem_ld_cols<W>(tmem + lane_base + (g & 1u) * N + col0 + c0, u);
+            tmem_ld_wait();
+#pragma unroll
+            for (int c = 0; c < W; ++c)
+              v[c] = pos < lim[col0 + c0 + c] ? __uint_as_float(u[c]) * scale_log2 : -INFINITY;
+            const float top = fold_columns<W>(v, lane, [](float x, float y) { return fmaxf(x, y); });
+            if (lane % (32 / W) == 0)
+              atomicMax(reinterpret_cast<unsigned int*>(corr) + col0 + c0 + lane * W / 32, float_key(top));
+          }
+          half_sync(half);
+          if (ht < NC) {
+            const float old = mref[col0 + ht], top = float_unkey(reinterpret_cast<uint32_t*>(corr)[col0 + ht]);
+            const float now = fmaxf(old, top);
+            mref[col0 + ht] = now;
+            corr[col0 + ht] = ex2_approx(old - now);
+          }
+          half_sync(half);
+#pragma unroll
+          for (int c = 0; c < NC; c += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(corr + col0 + c);
+            l[c] *= f.x;
+            l[c + 1] *= f.y;
+            l[c + 2] *= f.z;
+            l[c + 3] *= f.w;
+          }
+          if (t > w.t0) {   // the first tile of an item overwrites O^T
+            mbar_wait_bounded(pv_done, (g - 1) & 1u, abort_flag, status, DSV3_ERR_WAIT_TMEM);
+            tc_fence_after();
+#pragma unroll 1
+            for (int i = 0; i < pl.LP * (NC / 8); ++i) {
+              const int m = i / (NC / 8), c = i % (NC / 8) * 8;
+              uint32_t o[8];
+              tmem_ld8(tmem + lane_base + (2 + m) * N + col0 + c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr[col0 + c + j]);
+              tmem_st8(tmem + lane_base + (2 + m) * N + col0 + c, o);
+            }
+            tmem_st_wait();
+          }
+          half_sync(half);
+          if (ht < NC) reinterpret_cast<uint32_t*>(corr)[col0 + ht] = 0u;
         }
-        const bool move = half_any(half, over > 8.f);
         // P and O^T of the previous tile are no longer in use by the tensor core
         if (g > 0) mbar_wait_bounded(pv_done, (g - 1) & 1u, abort_flag, status, DSV3_ERR_WAIT_TMEM);
-        tc_fence_after();
-        if (move) {
-#pragma unroll
-          for (int c0 = 0; c0 < NC; c0 += 32) {
-            constexpr int W = NC < 32 ? NC : 32;
-            uint32_t mine = 0;
-#pragma unroll
-            for (int c = 0; c < W; ++c) {
-              const uint32_t k = __reduce_max_sync(0xffffffffu, float_key(__uint_as_float(sr[c0 + c]) * scale_log2));
-              if (lane == c) mine = k;
-            }
-            if (lane < W) myred[lane * 4 + (warp - 2 - 4 * half)] = float_unkey(mine);
-            half_sync(half);
-            float keep = kPaUnset;
-#pragma unroll
-            for (int c = 0; c < W; c += 8) {
-              float corr[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float4 r4 = *reinterpret_cast<const float4*>(myred + (c + i) * 4);
-                const float old = mref[col0 + c0 + c + i];
-                const float top = fmaxf(fmaxf(fmaxf(r4.x, r4.y), fmaxf(r4.z, r4.w)), old);
-                corr[i] = ex2_approx(old - top);
-                l[c0 + c + i] *= corr[i];
-                if (lane == c + i) keep = top;
-              }
-              if (t > w.t0) {
-                for (int m = 0; m < pl.LP; ++m) {
-                  uint32_t o[8];
-                  const uint32_t at = tmem + lane_base + (2 + m) * N + col0 + c0 + c;
-                  tmem_ld8(at, o);
-                  tmem_ld_wait();
-#pragma unroll
-                  for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr[i]);
-                  tmem_st8(at, o);
-                }
-              }
-            }
-            half_sync(half);                       // all threads have read the old references
-            if (ht < W) mref[col0 + c0 + lane] = keep;
-          }
-          tmem_st_wait();
-          half_sync(half);
-        }
         uint8_t* prow = smem + pl.off_p + key * 128;
 #pragma unroll
         for (int c = 0; c < NC; c += 8) {
-          uint32_t pk[4];
-#pragma unroll
-          for (int i = 0; i < 8; i += 4) {
-            const float4 m4 = mref4[(c + i) / 4];
-            const float p0 = ex2_approx(fmaf(__uint_as_float(sr[c + i]), scale_log2, -m4.x));
-            const float p1 = ex2_approx(fmaf(__uint_as_float(sr[c + i + 1]), scale_log2, -m4.y));
-            const float p2 = ex2_approx(fmaf(__uint_as_float(sr[c + i + 2]), scale_log2, -m4.z));
-            const float p3 = ex2_approx(fmaf(__uint_as_float(sr[c + i + 3]), scale_log2, -m4.w));
-            pk[i / 2] = pack_bf16x2(p0, p1);
-            pk[i / 2 + 1] = pack_bf16x2(p2, p3);
-            l[c + i] += __uint_as_float(pk[i / 2] << 16);
-            l[c + i + 1] += __uint_as_float(pk[i / 2] & 0xffff0000u);
-            l[c + i + 2] += __uint_as_float(pk[i / 2 + 1] << 16);
-            l[c + i + 3] += __uint_as_float(pk[i / 2 + 1] & 0xffff0000u);
-          }
           const int n = col0 + c;
           *reinterpret_cast<uint4*>(prow + (n >> 6) * kPaChunk + ((((n & 63) >> 3) ^ (key & 7)) << 4)) =
-              make_uint4(pk[0], pk[1], pk[2], pk[3]);
+              make_uint4(pk[c / 2], pk[c / 2 + 1], pk[c / 2 + 2], pk[c / 2 + 3]);
         }
         // rows of the pages past the cached length hold anything: zero them, so
         // that their zero weights do not meet an infinity or NaN
@@ -660,6 +769,12 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_ready);
+        // row sums over the rounded weights, while the tensor core runs
+#pragma unroll
+        for (int c = 0; c < NC; c += 2) {
+          l[c] += __uint_as_float(pk[c / 2] << 16);
+          l[c + 1] += __uint_as_float(pk[c / 2] & 0xffff0000u);
+        }
       }
       // ---- item epilogue
       mbar_wait_bounded(pv_done, (g - 1) & 1u, abort_flag, status, DSV3_ERR_WAIT_TMEM);
@@ -671,46 +786,39 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
         const long long s0 = start->first + (count - w.left);
         my_rec = make_int4((int)row0, nr, (int)((s0 + w.nt - 1) / start->share), 0);
       }
+      constexpr int W = NC < 32 ? NC : 32;
 #pragma unroll
-      for (int c0 = 0; c0 < NC; c0 += 32) {
-        constexpr int W = NC < 32 ? NC : 32;
+      for (int c0 = 0; c0 < NC; c0 += W) {
+        const float v = fold_columns<W>(*reinterpret_cast<float(*)[W]>(&l[c0]), lane,
+                                        [](float x, float y) { return x + y; });
+        if (c0 > 0) half_sync(half);               // the last group is read
+        if (lane % (32 / W) == 0) myred[lane * W / 32 * 4 + (warp - 2 - 4 * half)] = v;
         half_sync(half);
-#pragma unroll
-        for (int c = 0; c < W; ++c) {
-          const float v = warp_sum(l[c0 + c]);
-          if (lane == c) myred[c * 4 + (warp - 2 - 4 * half)] = v;
+        if (ht < W) {
+          const float4 r4 = *reinterpret_cast<const float4*>(myred + ht * 4);
+          const float sum = (r4.x + r4.y) + (r4.z + r4.w);
+          const int n = col0 + c0 + ht;
+          if (!whole) part_ml[(size_t)slot * N + n] = make_float2(mref[n], sum);
+          corr[n] = !whole ? 1.f : (sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum));
         }
-        half_sync(half);
-        if (!whole && ht < W) {
-          const float4 r4 = *reinterpret_cast<const float4*>(myred + lane * 4);
-          const int n = col0 + c0 + lane;
-          part_ml[(size_t)slot * N + n] = make_float2(mref[n], (r4.x + r4.y) + (r4.z + r4.w));
-        }
+      }
+      half_sync(half);
+#pragma unroll 1
+      for (int i = 0; i < pl.LP * (NC / 8); ++i) {
+        const int m = i / (NC / 8), n0 = col0 + i % (NC / 8) * 8;
+        const int r = 128 * m + key;
+        if (n0 >= nr) continue;
+        uint32_t o[8];
+        tmem_ld8(tmem + lane_base + (2 + m) * N + n0, o);
+        tmem_ld_wait();
+        if (r < R) {
 #pragma unroll
-        for (int c = 0; c < W; c += 8) {
-          float inv[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 r4 = *reinterpret_cast<const float4*>(myred + (c + i) * 4);
-            const float sum = (r4.x + r4.y) + (r4.z + r4.w);
-            inv[i] = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
-          }
-          for (int m = 0; m < pl.LP; ++m) {
-            uint32_t o[8];
-            tmem_ld8(tmem + lane_base + (2 + m) * N + col0 + c0 + c, o);
-            tmem_ld_wait();
-            const int r = 128 * m + key;
-            if (r < R) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int n = col0 + c0 + c + i;
-                if (n < nr) {
-                  if (whole) out[(size_t)(row0 + n) * R + r] = __float2bfloat16(__uint_as_float(o[i]) * inv[i]);
-                  else part_o[((size_t)slot * N + n) * R + r] = __uint_as_float(o[i]);
-                }
-              }
+          for (int j = 0; j < 8; ++j)
+            if (n0 + j < nr) {
+              const float v = __uint_as_float(o[j]) * corr[n0 + j];
+              if (whole) out[(size_t)(row0 + n0 + j) * R + r] = __float2bfloat16(v);
+              else part_o[((size_t)slot * N + n0 + j) * R + r] = v;
             }
-          }
         }
       }
       tc_fence_before();
@@ -726,7 +834,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
   }
 }
 
-// Joins the partials of row tiles that were cut: CTA (g, y) takes rows of the
+// Joins the partials of row tiles that were cut: CTA (g, y) takes row y of the
 // one that begins in share g.  The parts are added in share order.
 template <int N>
 __global__ void __launch_bounds__(128) paged_merge_kernel(const float* __restrict__ part_o,
