@@ -208,6 +208,8 @@ at::Tensor paged_latent_attention(const at::Tensor& q, const at::Tensor& pages, 
   const uint32_t kb[3] = {64, (uint32_t)std::min(rg.page, 128), 1};
   const CUtensorMap tm_kv = make_map(pages.data_ptr(), 3, kd, ks, kb);
   auto st = at::cuda::getCurrentCUDAStream();
+  const int64_t cuts = std::min<int64_t>(sms, T * H / N + rg.B);   // row tiles that can be cut, at most
+  const bool few = cuts * 4 <= sms;
   bf16* o = reinterpret_cast<bf16*>(out.data_ptr());
 #define DSV3_PAGED(N_)                                                                                           \
   do {                                                                                                           \
@@ -217,8 +219,10 @@ at::Tensor paged_latent_attention(const at::Tensor& q, const at::Tensor& pages, 
         tm_q, tm_kv, pl, rg, (int)T, (int)H, (int)R, (int)D, (float)(scale * 1.4426950408889634), 1, o, part, ml, \
         rec, status_ptr());                                                                                      \
     C10_CUDA_KERNEL_LAUNCH_CHECK();                                                                              \
-    paged_merge_kernel<N_><<<dim3(sms, N_), 128, 0, st>>>(part, ml, rec, (int)R, o);                             \
-    C10_CUDA_KERNEL_LAUNCH_CHECK();                                                                              \
+    C10_CUDA_CHECK(few ? launch_dependent(paged_merge_kernel<N_, true>, dim3((unsigned)cuts, N_), 512, st,       \
+                                          (const float*)part, (const float2*)ml, (const int4*)rec, sms, (int)R, o) \
+                       : launch_dependent(paged_merge_kernel<N_, false>, dim3(sms, N_ / 8), 256, st,             \
+                                          (const float*)part, (const float2*)ml, (const int4*)rec, sms, (int)R, o)); \
   } while (0)
   if (N == 16) DSV3_PAGED(16);
   else if (N == 32) DSV3_PAGED(32);

@@ -44,6 +44,7 @@ constexpr int kPaChunk = 128 * 128;          // [128 keys x 64 columns] bf16, by
 constexpr int kPaPair = 2 * kPaChunk;
 constexpr int kPaMaxSlots = 8;
 constexpr float kPaUnset = -1e30f;           // reference of a row that has seen no key
+constexpr float kPaLead = 12.f;              // first reference above the first key's score (log2)
 
 struct PagedPlan {
   int N, LP, nch, tail;       // row tile, latent chunk pairs, chunks, 1 if there is a tail chunk
@@ -166,15 +167,15 @@ template <int N>
 struct PagedWalk {
   const Ragged& r;
   int H, total;
-  long long left;
+  int left;
   int b, rt, t0, t1, nt;
   PagedSeq s;
-  __device__ __forceinline__ PagedWalk(const Ragged& r_, int H_, int total_, long long count, int b0, int rt0, int tile0)
+  __device__ __forceinline__ PagedWalk(const Ragged& r_, int H_, int total_, int count, int b0, int rt0, int tile0)
       : r(r_), H(H_), total(total_), left(count), b(b0), rt(rt0), t0(tile0) {
     if (left > 0) {
       s = paged_seq<N>(r, b, H, total);
       nt = paged_key_tiles<N>(s, rt, H);
-      t1 = (int)min((long long)nt, t0 + left);
+      t1 = min(nt, t0 + left);
     }
   }
   __device__ __forceinline__ bool ok() const { return left > 0; }
@@ -193,7 +194,7 @@ struct PagedWalk {
       } while (s.tiles == 0);
     }
     nt = paged_key_tiles<N>(s, rt, H);
-    t1 = (int)min((long long)nt, left);
+    t1 = min(nt, left);
   }
 };
 
@@ -245,25 +246,24 @@ __device__ __forceinline__ float float_unkey(uint32_t k) {
 
 // Start of this CTA's share, found by the whole CTA.
 struct PagedStart {
-  long long count;            // key tiles in the share
-  long long share;
-  long long first;            // flat index of its first key tile
-  long long local;            // its index within sequence b
-  int b, rt, tile;
+  int count;                  // key tiles in the share
+  int share;
+  int first;                  // flat index of its first key tile
+  int local;                  // its index within sequence b
+  int b, rt, tile, found;
 };
 
 template <int N>
-__device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, int min_share, PagedStart* out,
-                                           long long* scan, unsigned int* status) {
+__device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, int min_share, PagedStart* out, int* scan, unsigned int* status) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int NW = kPaThreads / 32;
   // round 0 adds up all sequences; round 1 finds the one that holds the share's
   // first tile (a batch of up to kPaThreads sequences is still in registers)
-  long long target = 0, t = 0;
+  int target = 0, t = 0;
   PagedSeq s;
   s.tiles = 0;
   for (int round = 0; round < 2; ++round) {
-    long long base = 0;
+    int base = 0;
     for (int b0 = 0; b0 < r.B; b0 += kPaThreads) {
       const int b = b0 + tid;
       if (round == 0 || r.B > kPaThreads) {
@@ -271,7 +271,7 @@ __device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, in
         t = 0;
         if (b < r.B) {
           s = paged_seq<N>(r, b, H, total);
-          t = paged_tiles_before<N>(s, s.tiles, H);
+          t = (int)paged_tiles_before<N>(s, s.tiles, H);
           if (round == 0 && blockIdx.x == 0) {
             const int c0 = __ldg(r.cu + b), c1 = __ldg(r.cu + b + 1);
             if (__ldg(r.lens + b) > r.cols * r.page || c1 > total || c1 < c0 || (b == 0 && c0 != 0) ||
@@ -280,30 +280,34 @@ __device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, in
           }
         }
       }
-      long long inc = t;
+      int inc = t;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+        const int v = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += v;
       }
       if (lane == 31) scan[warp] = inc;
       __syncthreads();
-      long long before = base, all = base;
+      int before = base, all = base;
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        const long long v = scan[w];
+        const int v = scan[w];
         if (w < warp) before += v;
         all += v;
       }
       if (round == 1 && t > 0 && before + inc - t <= target && target < before + inc) {
         out->b = b;
         out->local = target - (before + inc - t);
+        if (s.tiles == 1) {
+          out->tile = (int)out->local;
+          out->found = 1;
+        }
       }
       base = all;
       __syncthreads();
     }
     if (round == 0) {
-      long long share = (base + gridDim.x - 1) / gridDim.x;
+      int share = (base + gridDim.x - 1) / gridDim.x;
       if (share < min_share) share = min_share;
       target = share * blockIdx.x;
       if (tid == 0) {
@@ -312,13 +316,14 @@ __device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, in
         out->count = min(share, base - target);
         out->b = out->rt = out->tile = 0;
         out->local = 0;
+        out->found = 0;
       }
       if (target >= base) break;
     }
   }
   __syncthreads();
-  if (out->count > 0) {   // the row tile of that sequence: every thread tries one candidate
-    const long long local = out->local;
+  if (out->count > 0 && !out->found) {   // the row tile of that sequence: every thread tries one candidate
+    const int local = out->local;
     s = paged_seq<N>(r, out->b, H, total);
     int lo = 0, hi = s.tiles;                    // the answer lies in [lo, hi)
     while (hi > lo) {
@@ -434,7 +439,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
   uint64_t* o_free = pv_done + 1;
   uint64_t* drain = o_free + 1;
   PagedStart* start = reinterpret_cast<PagedStart*>(drain + 1);
-  long long* scan = reinterpret_cast<long long*>(start + 1);             // [kPaThreads / 32]
+  int* scan = reinterpret_cast<int*>(start + 1);             // [kPaThreads / 32]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(scan + kPaThreads / 32);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -465,12 +470,13 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
     tmem_alloc(tmem_slot, pl.tmem_cols);
     tmem_relinquish();
   }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   paged_find<N>(rg, H, total, min_share, start, scan, status);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const long long count = start->count;
+  const int count = start->count;
   const uint32_t smem0 = smem_u32(smem);
   const int boxes = rg.page >= 128 ? 1 : 128 / rg.page;        // TMA boxes per chunk
 
@@ -652,7 +658,6 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
       half_sync(half);                             // the last item's references are read
       if (ht < NC) {
         const int n = col0 + ht;
-        mref[n] = kPaUnset;
         reinterpret_cast<uint32_t*>(corr)[n] = 0u;
         lim[n] = n < nr ? base + (w.rt * N + n) / H + 1 : 0;
       }
@@ -677,6 +682,25 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
             if (pos >= k4.z) sr[c + 2] = 0xff800000u;
             if (pos >= k4.w) sr[c + 3] = 0xff800000u;
           }
+        }
+        // The first references are the scores of the tile's first key plus 12:
+        // scores up to 2^20 times its weight pass without a move, and weights
+        // lose nothing by starting at 2^-12 (a maximum over the tile first cost
+        // 1,700 to 8,000 cycles per item).  A row that does not see that key
+        // sees none of this tile.
+        if (t == w.t0) {
+          if (key == 0) {
+#pragma unroll
+            for (int c = 0; c < NC; c += 4) {
+              float4 m4;
+              m4.x = fmaxf(fmaf(__uint_as_float(sr[c]), scale_log2, kPaLead), kPaUnset);
+              m4.y = fmaxf(fmaf(__uint_as_float(sr[c + 1]), scale_log2, kPaLead), kPaUnset);
+              m4.z = fmaxf(fmaf(__uint_as_float(sr[c + 2]), scale_log2, kPaLead), kPaUnset);
+              m4.w = fmaxf(fmaf(__uint_as_float(sr[c + 3]), scale_log2, kPaLead), kPaUnset);
+              mref4[c / 4] = m4;
+            }
+          }
+          half_sync(half);
         }
         // p = 2^(s - m) at the present references; where one is passed by more
         // than 2^8 the half moves them and computes p again
@@ -762,7 +786,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
             const int slot = (g * pl.LP + (c >> 1)) % pl.slots;
             uint4* z = reinterpret_cast<uint4*>(smem + slot * kPaPair + (c & 1) * kPaChunk + key * 128);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) z[i] = make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < 8; ++i) z[(i + lane) & 7] = make_uint4(0, 0, 0, 0);   // spread over the banks
           }
         }
         fence_proxy_async_smem();
@@ -783,8 +807,8 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
       const int slot = 2 * blockIdx.x + (w.t0 == 0 ? 1 : 0);
       const long long row0 = (long long)w.s.tok0 * H + (long long)w.rt * N;
       if (!whole && w.t0 == 0) {
-        const long long s0 = start->first + (count - w.left);
-        my_rec = make_int4((int)row0, nr, (int)((s0 + w.nt - 1) / start->share), 0);
+        const int s0 = start->first + (count - w.left);
+        my_rec = make_int4((int)row0, nr, (s0 + w.nt - 1) / start->share, 0);
       }
       constexpr int W = NC < 32 ? NC : 32;
 #pragma unroll
@@ -803,22 +827,32 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
         }
       }
       half_sync(half);
+      // O^T out: a thread holds one latent column of W rows; finished rows are
+      // exchanged between neighbouring lanes and stored as bf16 pairs
 #pragma unroll 1
-      for (int i = 0; i < pl.LP * (NC / 8); ++i) {
-        const int m = i / (NC / 8), n0 = col0 + i % (NC / 8) * 8;
+      for (int i = 0; i < pl.LP * (NC / W); ++i) {
+        const int m = i / (NC / W), n0 = col0 + i % (NC / W) * W;
         const int r = 128 * m + key;
         if (n0 >= nr) continue;
-        uint32_t o[8];
-        tmem_ld8(tmem + lane_base + (2 + m) * N + n0, o);
+        uint32_t o[W];
+        tmem_ld_cols<W>(tmem + lane_base + (2 + m) * N + n0, o);
         tmem_ld_wait();
-        if (r < R) {
+        if (whole) {
+          const bool odd = lane & 1;
+          bf16* at = out + (size_t)(row0 + n0 + odd) * R + (r & ~1);
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (n0 + j < nr) {
-              const float v = __uint_as_float(o[j]) * corr[n0 + j];
-              if (whole) out[(size_t)(row0 + n0 + j) * R + r] = __float2bfloat16(v);
-              else part_o[((size_t)slot * N + n0 + j) * R + r] = v;
-            }
+          for (int j = 0; j < W; j += 2) {
+            const float2 f = *reinterpret_cast<const float2*>(corr + n0 + j);
+            const float x = __uint_as_float(o[j]) * f.x, y = __uint_as_float(o[j + 1]) * f.y;
+            const float got = __shfl_xor_sync(0xffffffffu, odd ? x : y, 1);
+            const uint32_t v = odd ? pack_bf16x2(got, y) : pack_bf16x2(x, got);
+            if (r < R && n0 + j + odd < nr) *reinterpret_cast<uint32_t*>(at + (size_t)j * R) = v;
+          }
+        } else if (r < R) {
+          float* at = part_o + ((size_t)slot * N + n0) * R + r;
+#pragma unroll
+          for (int j = 0; j < W; ++j)
+            if (n0 + j < nr) at[(size_t)j * R] = __uint_as_float(o[j]);
         }
       }
       tc_fence_before();
@@ -834,46 +868,116 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
   }
 }
 
-// Joins the partials of row tiles that were cut: CTA (g, y) takes row y of the
-// one that begins in share g.  The parts are added in share order.
-template <int N>
-__global__ void __launch_bounds__(128) paged_merge_kernel(const float* __restrict__ part_o,
-                                                          const float2* __restrict__ part_ml,
-                                                          const int4* __restrict__ rec, int R,
-                                                          bf16* __restrict__ out) {
-  const int g = blockIdx.x;
+// Joins the partials of row tiles that were cut.  rec[g] describes the one that
+// begins in share g and goes on: part 0 is slot 2 g + 1, part i slot 2 (g + i).
+// The parts are added in a fixed order.  Where shares outnumber row tiles (few
+// rows over long contexts, FEW) a CTA joins one row, its threads split over the
+// parts; else a warp joins one row, of two or three parts as a rule.
+template <int N, bool FEW>
+__global__ void __launch_bounds__(FEW ? 512 : 256) paged_merge_kernel(const float* __restrict__ part_o,
+                                                                    const float2* __restrict__ part_ml,
+                                                                    const int4* __restrict__ rec, int shares, int R,
+                                                                    bf16* __restrict__ out) {
+  __shared__ int s_g;
+  __shared__ float s_m[32];
+  __shared__ float4 s_acc[FEW ? 512 : 1];
+  __shared__ float s_sum[FEW ? 256 : 1];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int g = blockIdx.x, n;
+  if constexpr (FEW) {
+    // the blockIdx.x-th row tile that was cut
+    if (warp == 0) {
+      int skip = blockIdx.x, found = -1;
+      for (int i = 0; i < shares && found < 0; i += 32) {
+        const unsigned hit = __ballot_sync(0xffffffffu, i + lane < shares && rec[min(i + lane, shares - 1)].x >= 0);
+        const int c = __popc(hit);
+        if (skip < c) {
+          const bool me = (hit >> lane & 1) && __popc(hit & ((1u << lane) - 1)) == skip;
+          found = i + __ffs(__ballot_sync(0xffffffffu, me)) - 1;
+        }
+        skip -= c;
+      }
+      if (lane == 0) s_g = found;
+    }
+    __syncthreads();
+    g = s_g;
+    if (g < 0) return;
+    n = blockIdx.y;
+  } else {
+    n = blockIdx.y * 8 + warp;
+  }
   const int4 rc = rec[g];
-  const int n = blockIdx.y;
   if (rc.x < 0 || n >= rc.y) return;
   const int parts = rc.z - g + 1;
-  // part 0 is slot 2 g + 1, part i > 0 slot 2 (g + i)
+  auto at = [&](int i) { return (size_t)(i ? 2 * (g + i) : 2 * g + 1) * N + n; };
   float M = -INFINITY;
-  for (int i = 0; i < parts; ++i) {
-    const float2 ml = part_ml[(size_t)(i ? 2 * (g + i) : 2 * g + 1) * N + n];
+  for (int i = FEW ? tid : lane; i < parts; i += FEW ? 512 : 32) {
+    const float2 ml = part_ml[at(i)];
     if (ml.y > 0.f) M = fmaxf(M, ml.x);
   }
-  float sum = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  const int r = threadIdx.x * 4;
-  for (int i = 0; i < parts; ++i) {
-    const size_t at = (size_t)(i ? 2 * (g + i) : 2 * g + 1) * N + n;
-    const float2 ml = part_ml[at];
-    if (ml.y == 0.f) continue;
-    const float wgt = ex2_approx(ml.x - M);
-    sum += ml.y * wgt;
-    if (r < R) {
-      const float4 o = *reinterpret_cast<const float4*>(part_o + at * R + r);
-      acc.x += o.x * wgt;
-      acc.y += o.y * wgt;
-      acc.z += o.z * wgt;
-      acc.w += o.w * wgt;
-    }
+  M = warp_max(M);
+  // threads of one part: R / 4 of them hold four latent columns each
+  const int tpp = FEW ? R / 4 : 32, groups = FEW ? 512 / tpp : 1, grp = FEW ? tid / tpp : 0;
+  if constexpr (FEW) {
+    if (lane == 0) s_m[warp] = M;
+    __syncthreads();
+    M = s_m[lane & 15];
+    M = warp_max(M);
   }
-  if (r < R) {
+  for (int r = FEW ? (tid % tpp) * 4 : lane * 4; r < R; r += FEW ? R : 128) {
+    float sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (grp < groups) {
+#pragma unroll 4
+      for (int i = grp; i < parts; i += groups) {
+        const size_t k = at(i);
+        const float2 ml = part_ml[k];
+        const float4 o = *reinterpret_cast<const float4*>(part_o + k * R + r);
+        const float wgt = ml.y == 0.f ? 0.f : ex2_approx(ml.x - M);
+        sum += ml.y * wgt;
+        if (wgt != 0.f) {
+          acc.x += o.x * wgt;
+          acc.y += o.y * wgt;
+          acc.z += o.z * wgt;
+          acc.w += o.w * wgt;
+        }
+      }
+    }
+    if constexpr (FEW) {
+      s_acc[tid] = acc;
+      if (tid % tpp == 0 && grp < groups) s_sum[grp] = sum;
+      __syncthreads();
+      if (grp > 0) return;
+      for (int i = 1; i < groups; ++i) {
+        const float4 o = s_acc[i * tpp + tid];
+        acc.x += o.x;
+        acc.y += o.y;
+        acc.z += o.z;
+        acc.w += o.w;
+        sum += s_sum[i];
+      }
+    }
     const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
     uint2 v;
     v.x = pack_bf16x2(acc.x * inv, acc.y * inv);
     v.y = pack_bf16x2(acc.z * inv, acc.w * inv);
     *reinterpret_cast<uint2*>(out + (size_t)(rc.x + n) * R + r) = v;
   }
+}
+
+// Launch that may begin while its predecessor in the stream still runs; the
+// kernel waits for it (griddepcontrol.wait) before it reads anything.
+template <typename Kern, typename... Args>
+inline cudaError_t launch_dependent(Kern kern, dim3 grid, int block, cudaStream_t st, Args... args) {
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
 }
