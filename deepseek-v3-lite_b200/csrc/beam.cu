@@ -6,6 +6,7 @@
 #include <tuple>
 
 #include "common.cuh"
+#include "launch.h"
 #include "status.h"
 
 namespace dsv3 {
@@ -15,9 +16,9 @@ namespace {
 typedef __nv_bfloat16 bf16;
 
 constexpr int kMaxBeams = 32;
-constexpr int kSelThreads = 256;
-constexpr int kSelPer = 32;                        // logits per thread
-constexpr int kSelSeg = kSelThreads * kSelPer;     // logits per CTA
+constexpr int kScanThreads = 256;
+constexpr int kPickThreads = 512;
+constexpr int kListCap = 512;      // candidates at or above a CTA's threshold that it ranks in shared memory
 
 // Order-preserving map of a float to an unsigned key (larger float, larger
 // key); 0 stands for "no candidate" and lies below the key of -inf.
@@ -28,233 +29,308 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
 }
+// (key, index) as one number: a larger one is the better candidate, that is the
+// larger value, and of equal values the lower index.
+__device__ __forceinline__ uint64_t entry_of(uint32_t key, uint32_t index) { return (uint64_t)key << 32 | ~index; }
+__device__ __forceinline__ uint32_t entry_index(uint64_t e) { return ~(uint32_t)e; }
 
 // A logit as the selection sees it: NaN counts as -inf, +inf as the largest
 // finite float, so that the log-sum-exp of a row is always defined.
 __device__ __forceinline__ float clean_logit(float x) { return fminf(fmaxf(x, -INFINITY), 3.402823466e38f); }
-__device__ __forceinline__ float load_logit(const float* p) { return clean_logit(*p); }
-__device__ __forceinline__ float load_logit(const bf16* p) { return clean_logit(__bfloat162float(*p)); }
+__device__ __forceinline__ float clean_logit(bf16 x) { return clean_logit(__bfloat162float(x)); }
 
-// Top `k` of (key, index) pairs held by a warp, `n` per lane: larger key first, ties to the lower index.
-// Lane 0 emits through `put(rank, key, index)`.
-template <int N, typename Put>
-__device__ __forceinline__ void warp_top(uint32_t (&key)[N], const uint32_t (&idx)[N], int k, int lane, Put put) {
-  for (int j = 0; j < k; ++j) {
-    uint32_t bk = 0, bi = 0xffffffffu;
+// The k best of a CTA's candidates.  The r-th largest of the lane maxima of each
+// warp, r = ceil(k / warps), is below at least k candidates, and so is the
+// smallest of these over the warps, the threshold: few candidates reach it
+// (22 of 8,192 for k = 8 on random data), and these are ranked by counting.
+// `top` is the lane's largest key, `each(f)` calls f(entry) for every candidate
+// of the thread.  Where more reach it than the list holds (many equal values) the
+// best are taken one at a time.  put(rank, entry) is called once per rank; a rank
+// without a candidate gets 0.
+template <int THREADS, typename Each, typename Put>
+__device__ __forceinline__ void cta_best(int k, uint32_t top, Each each, Put put) {
+  constexpr int W = THREADS / 32;
+  __shared__ uint32_t s_low[W];
+  __shared__ uint64_t s_list[kListCap];
+  __shared__ int s_n;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint32_t left = top, low = 0;
+  for (int i = 0; i < (k + W - 1) / W; ++i) {
+    low = __reduce_max_sync(0xffffffffu, left);
+    const unsigned who = __ballot_sync(0xffffffffu, left == low);
+    if (lane == __ffs(who) - 1) left = 0;
+  }
+  if (lane == 0) s_low[warp] = low;
+  if (tid == 0) s_n = 0;
+  __syncthreads();
+  uint32_t threshold = s_low[0];
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (key[i] > bk || (key[i] == bk && idx[i] < bi)) {
-        bk = key[i];
-        bi = idx[i];
+  for (int w = 1; w < W; ++w) threshold = min(threshold, s_low[w]);
+  if (top >= threshold && top > 0)
+    each([&](uint64_t e) {
+      if ((uint32_t)(e >> 32) >= threshold && e >> 32) {
+        const int at = atomicAdd(&s_n, 1);
+        if (at < kListCap) s_list[at] = e;
       }
-    const uint32_t top = __reduce_max_sync(0xffffffffu, bk);
-    const uint32_t at = __reduce_min_sync(0xffffffffu, bk == top ? bi : 0xffffffffu);
-    if (lane == 0) put(j, top, at);
+    });
+  __syncthreads();
+  const int n = s_n;
+  if (n <= kListCap) {
+    for (int i = tid; i < n; i += THREADS) {
+      const uint64_t e = s_list[i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += s_list[j] > e;
+      if (rank < k) put(rank, e);
+    }
+    for (int i = n + tid; i < k; i += THREADS) put(i, (uint64_t)0);
+    return;
+  }
+  uint64_t last = ~(uint64_t)0;
+  for (int r = 0; r < k; ++r) {
+    uint64_t best = 0;
+    each([&](uint64_t e) {
+      if (e < last && e > best) best = e;
+    });
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (idx[i] == at) key[i] = 0;
+    for (int o = 16; o > 0; o >>= 1) {
+      const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
+      if (other > best) best = other;
+    }
+    __syncthreads();                     // the last round's entries are read
+    if (lane == 0) s_list[warp] = best;
+    __syncthreads();
+    for (int w = 0; w < W; ++w)
+      if (s_list[w] > best) best = s_list[w];
+    if (tid == 0) put(r, best);
+    last = best;
   }
 }
 
-// One CTA per (segment of a row): maximum, sum of exponentials and the `k` largest logits.
-template <typename T>
-__global__ void __launch_bounds__(kSelThreads) beam_scan_kernel(const T* __restrict__ logits, long ldb, long ldk, int K,
-                                                                int V, int k, const bool* __restrict__ finished,
-                                                                float2* __restrict__ stat,
-                                                                uint2* __restrict__ cand) {
+// 16 bytes at an address that is `align` (0, 4, 8 or 12) modulo 16.
+__device__ __forceinline__ uint4 load_16_bytes(const void* p, int align) {
+  if (align == 0) return __ldg(reinterpret_cast<const uint4*>(p));
+  uint4 u;
+  if (align == 8) {
+    const uint2 a = __ldg(reinterpret_cast<const uint2*>(p)), b = __ldg(reinterpret_cast<const uint2*>(p) + 1);
+    u = make_uint4(a.x, a.y, b.x, b.y);
+  } else {
+    const uint32_t* q = reinterpret_cast<const uint32_t*>(p);
+    u = make_uint4(__ldg(q), __ldg(q + 1), __ldg(q + 2), __ldg(q + 3));
+  }
+  return u;
+}
+
+// One CTA per (segment, row): maximum, sum of exponentials and the k largest of
+// PER * 256 logits, which stay in registers between one read and the rest.  A
+// thread's elements go by their index in the row, never by its address, so that
+// sums and scores are the same wherever a row lies.  Bound by reading the
+// logits (32 x 8 rows of 102,400 fp32: 16 us at the copy rate).
+template <typename T, int PER>
+__global__ void __launch_bounds__(kScanThreads) beam_scan_kernel(const T* __restrict__ logits, long ldb, long ldk, int K,
+                                                                 int V, const bool* __restrict__ finished,
+                                                                 float2* __restrict__ stat,
+                                                                 uint64_t* __restrict__ cand) {
+  constexpr int VE = 16 / sizeof(T), NV = PER / VE;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int row = blockIdx.y, seg = blockIdx.x, nseg = gridDim.x;
   if (finished != nullptr && finished[row]) return;
   const T* x = logits + (row / K) * ldb + (row % K) * ldk;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  __shared__ float red[2][kSelThreads / 32];
-  __shared__ uint2 top_s[kSelThreads / 32][kMaxBeams];
-  uint32_t key[kSelPer], idx[kSelPer];
-  float mx = -3.402823466e38f;
+  const int align = (int)(reinterpret_cast<uintptr_t>(x) & 15);
+  const int first = seg * PER * kScanThreads + tid * VE;
+  float v[PER];
 #pragma unroll
-  for (int i = 0; i < kSelPer; ++i) {
-    const int v = seg * kSelSeg + i * kSelThreads + tid;
-    idx[i] = v < V ? v : 0xfffffffeu;
-    const float f = v < V ? load_logit(x + v) : -INFINITY;
-    key[i] = v < V ? order_key(f) : 0;
-    mx = fmaxf(mx, f);
+  for (int j = 0; j < NV; ++j) {
+    const int at = first + j * kScanThreads * VE;
+    if (at + VE <= V && align % 4 == 0) {
+      const uint4 u = load_16_bytes(x + at, align);
+      const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) v[j * VE + i] = clean_logit(e[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VE; ++i) v[j * VE + i] = at + i < V ? clean_logit(x[at + i]) : -INFINITY;
+    }
   }
-  mx = warp_max(mx);
+  __shared__ float red[2][kScanThreads / 32];
+  float tmax = v[0];
+#pragma unroll
+  for (int i = 1; i < PER; ++i) tmax = fmaxf(tmax, v[i]);
+  float mx = warp_max(tmax);
   if (lane == 0) red[0][warp] = mx;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kSelThreads / 32; ++i) mx = fmaxf(mx, red[0][i]);
+  for (int i = 0; i < kScanThreads / 32; ++i) mx = fmaxf(mx, red[0][i]);
+  mx = fmaxf(mx, -3.402823466e38f);
   float s = 0.f;
 #pragma unroll
-  for (int i = 0; i < kSelPer; ++i) s += key[i] ? __expf(key_value(key[i]) - mx) : 0.f;
+  for (int i = 0; i < PER; ++i) s += __expf(v[i] - mx);
   s = warp_sum(s);
   if (lane == 0) red[1][warp] = s;
-  warp_top(key, idx, k, lane, [&](int j, uint32_t kk, uint32_t ii) { top_s[warp][j] = make_uint2(kk, ii); });
-  __syncthreads();
-  if (warp == 0) {
-    uint32_t k2[kMaxBeams / 4], i2[kMaxBeams / 4];
+  uint64_t* o = cand + ((size_t)row * nseg + seg) * K;
+  cta_best<kScanThreads>(
+      K, first < V ? order_key(tmax) : 0u,
+      [&](auto&& f) {
 #pragma unroll
-    for (int i = 0; i < kMaxBeams / 4; ++i) {
-      const int e = i * 32 + lane, w = e / k;
-      k2[i] = w < kSelThreads / 32 ? top_s[w][e % k].x : 0;
-      i2[i] = w < kSelThreads / 32 ? top_s[w][e % k].y : 0xfffffffeu;
-    }
-    uint2* o = cand + ((size_t)row * nseg + seg) * k;
-    warp_top(k2, i2, k, lane, [&](int j, uint32_t kk, uint32_t ii) { o[j] = make_uint2(kk, ii); });
-    if (lane == 0) {
-      float t = 0.f;
-      for (int i = 0; i < kSelThreads / 32; ++i) t += red[1][i];
-      stat[(size_t)row * nseg + seg] = make_float2(mx, t);
-    }
+        for (int i = 0; i < PER; ++i) {
+          const int at = first + (i / VE) * kScanThreads * VE + i % VE;
+          if (at < V) f(entry_of(order_key(v[i]), (uint32_t)at));
+        }
+      },
+      [&](int rank, uint64_t e) { o[rank] = e; });
+  if (tid == 0) {                         // the barriers of cta_best lie between
+    float t = 0.f;
+    for (int i = 0; i < kScanThreads / 32; ++i) t += red[1][i];
+    stat[(size_t)row * nseg + seg] = make_float2(mx, t);
   }
 }
 
 // One CTA per batch entry: log-sum-exp of its beams, then the K best candidates.
-__global__ void __launch_bounds__(256) beam_pick_kernel(const float2* __restrict__ stat, const uint2* __restrict__ cand,
-                                                        const float* __restrict__ scores,
-                                                        const bool* __restrict__ finished, int K, int V, int nseg,
-                                                        int eos, float* __restrict__ o_score, int* __restrict__ o_parent,
-                                                        int* __restrict__ o_token, bool* __restrict__ o_done) {
+__global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const float2* __restrict__ stat,
+                                                                 const uint64_t* __restrict__ cand,
+                                                                 const float* __restrict__ scores,
+                                                                 const bool* __restrict__ finished, int K, int V,
+                                                                 int nseg, int eos, float* __restrict__ o_score,
+                                                                 int* __restrict__ o_parent, int* __restrict__ o_token,
+                                                                 bool* __restrict__ o_done) {
   const int b = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  __shared__ float s_max[kMaxBeams], s_log[kMaxBeams];
-  __shared__ uint32_t s_key[8], s_at[8];
-  for (int r = warp; r < K; r += 8) {
-    const size_t row = (size_t)b * K + r;
+  __shared__ float s_max[kMaxBeams], s_log[kMaxBeams], s_score[kMaxBeams];
+  __shared__ bool s_done[kMaxBeams];
+  const size_t row0 = (size_t)b * K;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int r = warp; r < K; r += kPickThreads / 32) {
+    const bool done = finished != nullptr && finished[row0 + r];
+    const float2* st = stat + (row0 + r) * nseg;
     float m = -3.402823466e38f, s = 0.f;
-    if (!(finished != nullptr && finished[row])) {
-      for (int i = lane; i < nseg; i += 32) m = fmaxf(m, stat[row * nseg + i].x);
+    if (!done) {
+      for (int i = lane; i < nseg; i += 32) m = fmaxf(m, st[i].x);
       m = warp_max(m);
-      for (int i = lane; i < nseg; i += 32) s += stat[row * nseg + i].y * expf(stat[row * nseg + i].x - m);
+      for (int i = lane; i < nseg; i += 32) s += st[i].y * expf(st[i].x - m);
       s = warp_sum(s);
     }
     if (lane == 0) {
       s_max[r] = m;
       s_log[r] = logf(s);
+      s_score[r] = scores[row0 + r];
+      s_done[r] = done;
     }
   }
   __syncthreads();
-  const int per = nseg * K;       // candidates per beam
-  uint32_t last_key = 0xffffffffu, last_at = 0;
-  for (int j = 0; j < K; ++j) {
-    // best candidate after (last_key, last_at) in the order (key descending, flat index ascending)
-    uint32_t bk = 0, bi = 0xffffffffu;
-    for (int c = tid; c < K * per; c += 256) {
-      const int r = c / per, i = c % per;
-      const size_t row = (size_t)b * K + r;
-      const float sc = scores[row];
-      uint32_t v;
-      float val;
-      if (finished != nullptr && finished[row]) {
-        if (i >= K) continue;
-        v = i == 0 ? eos : (i - 1 < eos ? i - 1 : i);
-        val = i == 0 ? sc : -INFINITY;
-      } else if (!(sc > -INFINITY) || s_log[r] == -INFINITY) {
-        if (i >= K) continue;
-        v = i;
-        val = -INFINITY;
-      } else {
-        const uint2 e = cand[row * per + i];
-        if (e.x == 0) continue;
-        v = e.y;
-        val = sc + ((key_value(e.x) - s_max[r]) - s_log[r]);
-      }
-      if (v >= V) continue;
-      const uint32_t k2 = order_key(val), at = r * V + v;
-      const bool after = k2 < last_key || (k2 == last_key && at > last_at);
-      if (after && (k2 > bk || (k2 == bk && at < bi))) {
-        bk = k2;
-        bi = at;
-      }
+  const int per = nseg * K;               // candidates per beam
+  auto candidate = [&](int c) -> uint64_t {
+    const int r = c / per, i = c % per;
+    const float sc = s_score[r];
+    uint32_t v;
+    float val = -INFINITY;
+    if (s_done[r]) {                      // the end token at the unchanged score, others at -inf
+      if (i >= K) return 0;
+      v = i == 0 ? eos : (i - 1 < eos ? i - 1 : i);
+      if (i == 0) val = sc;
+    } else if (!(sc > -INFINITY) || s_log[r] == -INFINITY) {
+      if (i >= K) return 0;
+      v = i;
+    } else {
+      const uint64_t e = cand[row0 * per + c];
+      if (e == 0) return 0;
+      v = entry_index(e);
+      val = sc + ((key_value((uint32_t)(e >> 32)) - s_max[r]) - s_log[r]);
     }
-    const uint32_t wk = __reduce_max_sync(0xffffffffu, bk);
-    const uint32_t wi = __reduce_min_sync(0xffffffffu, bk == wk ? bi : 0xffffffffu);
-    if (lane == 0) {
-      s_key[warp] = wk;
-      s_at[warp] = wi;
-    }
-    __syncthreads();
-    last_key = 0;
-    last_at = 0xffffffffu;
-    for (int w = 0; w < 8; ++w)
-      if (s_key[w] > last_key || (s_key[w] == last_key && s_at[w] < last_at)) {
-        last_key = s_key[w];
-        last_at = s_at[w];
-      }
-    __syncthreads();
-    if (tid == 0) {
-      const int p = last_at / V, v = last_at % V;
-      o_score[b * K + j] = key_value(last_key);
-      o_parent[b * K + j] = p;
-      o_token[b * K + j] = v;
-      o_done[b * K + j] = (finished != nullptr && finished[(size_t)b * K + p]) || v == eos;
-    }
-  }
+    return v < (uint32_t)V ? entry_of(order_key(val), r * V + v) : 0;
+  };
+  uint32_t top = 0;
+  for (int c = tid; c < K * per; c += kPickThreads) top = max(top, (uint32_t)(candidate(c) >> 32));
+  cta_best<kPickThreads>(
+      K, top,
+      [&](auto&& f) {
+        for (int c = tid; c < K * per; c += kPickThreads) f(candidate(c));
+      },
+      [&](int rank, uint64_t e) {
+        const uint32_t at = entry_index(e);
+        const int p = at / V, v = at % V;
+        o_score[row0 + rank] = key_value((uint32_t)(e >> 32));
+        o_parent[row0 + rank] = p;
+        o_token[row0 + rank] = v;
+        o_done[row0 + rank] = s_done[p] || v == eos;
+      });
 }
 
-// Grid (part, layer, group): part < parts copies its share of the page that is
-// being filled, part == parts (layer 0 only) writes the group's new table rows.
-__global__ void __launch_bounds__(256) beam_reorder_kernel(uint4* __restrict__ pages, long ld_layer, long ld_page,
-                                                           int row16, int page, int pool, const int* __restrict__ table,
-                                                           long ldt, int cols, const int* __restrict__ parents, int K,
-                                                           const int* __restrict__ lens, int* __restrict__ out,
-                                                           int parts, unsigned int* status) {
-  __shared__ int s_src[kMaxBeams], s_dst[kMaxBeams], s_par[kMaxBeams], s_n;
-  const int b = blockIdx.z, layer = blockIdx.y, part = blockIdx.x;
-  if (part == parts && layer > 0) return;
+// Grid (x, layer, group).  CTA x < parts * splits copies 16 KB of the page that
+// is being filled, for every splits-th copy of its group; the last x (layer 0
+// only) writes the group's new table rows.  Bound by the copied bytes.
+constexpr int kCopyThreads = 256, kCopyVecs = 4;
+
+__global__ void __launch_bounds__(kCopyThreads) beam_reorder_kernel(uint4* __restrict__ pages, long ld_layer, long ld_page,
+                                                                    int row16, int page, int pool,
+                                                                    const int* __restrict__ table, long ldt, int cols,
+                                                                    const int* __restrict__ parents, int K,
+                                                                    const int* __restrict__ lens, int* __restrict__ out,
+                                                                    int parts, int splits, unsigned int* status) {
+  __shared__ int s_src[kMaxBeams], s_dst[kMaxBeams], s_par[kMaxBeams], s_cur[kMaxBeams], s_spare[kMaxBeams], s_n;
+  const int b = blockIdx.z, layer = blockIdx.y;
+  const bool writes_table = (int)blockIdx.x == parts * splits;
+  if (writes_table && layer > 0) return;
   const int len = lens[b];
   const int col = len / page, rem = len % page;
-  if (part < parts && rem == 0) return;
+  const int part = blockIdx.x % parts, split = blockIdx.x / parts;
+  const int n16 = rem * row16;
+  const int first = part * kCopyThreads * kCopyVecs + threadIdx.x;
+  if (!writes_table && part * kCopyThreads * kCopyVecs >= n16) return;
   const int* tb = table + (size_t)b * K * ldt;
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
-    int p = lane < K ? parents[b * K + lane] : -1;
-    bool bad = lane < K && (p < 0 || p >= K);
-    if (bad) p = lane;
-    int cur = lane < K && col < cols ? tb[lane * ldt + col] : -1;
-    if (lane < K && rem > 0 && (cur < 0 || cur >= pool)) bad = true;
-    if (bad) record_error(status, DSV3_ERR_BOUNDS);
-    const bool ok = !__any_sync(0xffffffffu, lane < K && rem > 0 && (cur < 0 || cur >= pool));
-    // children of the same parent; the first keeps its page, the j-th other takes the j-th childless beam's
-    const unsigned mine = __match_any_sync(0xffffffffu, p) & (K == 32 ? 0xffffffffu : (1u << K) - 1);
-    const bool again = lane < K && (mine & ((1u << lane) - 1)) != 0;
-    unsigned has = __reduce_or_sync(0xffffffffu, lane < K ? 1u << p : 0u);
-    const unsigned dead = ~has & (K == 32 ? 0xffffffffu : (1u << K) - 1);
-    const unsigned agains = __ballot_sync(0xffffffffu, again);
-    const int j = __popc(agains & ((1u << lane) - 1));
-    const int from = p < 0 ? 0 : p;
-    const int src = __shfl_sync(0xffffffffu, cur, from);
-    const int spare = again ? __fns(dead, 0, j + 1) : from;
-    const int dst = __shfl_sync(0xffffffffu, cur, spare);
-    if (lane < K) {
+    const bool beam = lane < K;
+    int p = beam ? parents[b * K + lane] : -1;
+    const int cur = beam && col < cols ? tb[lane * ldt + col] : -1;
+    const bool bad_parent = beam && (p < 0 || p >= K);
+    const bool bad_page = beam && rem > 0 && (cur < 0 || cur >= pool);
+    if (bad_parent) p = lane;
+    if (bad_parent || bad_page) record_error(status, DSV3_ERR_BOUNDS);
+    // the first child of a parent keeps its page, the j-th of the further
+    // children takes that of the j-th beam without a child
+    const unsigned below = (1u << lane) - 1;
+    const unsigned alike = __match_any_sync(0xffffffffu, p);     // all lanes take part
+    const bool again = beam && (alike & below) != 0;
+    const unsigned has = __reduce_or_sync(0xffffffffu, beam ? 1u << p : 0u);
+    const bool dead = beam && !(has >> lane & 1);
+    const unsigned agains = __ballot_sync(0xffffffffu, again), deads = __ballot_sync(0xffffffffu, dead);
+    const bool ok = !__any_sync(0xffffffffu, bad_page);
+    s_cur[lane] = cur;
+    if (dead) s_spare[__popc(deads & below)] = cur;
+    __syncwarp();
+    const int j = __popc(agains & below);
+    if (beam) {
+      const int src = s_cur[p], dst = again ? s_spare[j] : src;
       s_par[lane] = p;
-      s_dst[lane] = dst;
+      s_dst[lane] = dst;                  // by child, for the table
+      if (again) s_src[j] = src;
     }
     __syncwarp();
-    if (part < parts) {
-      if (again) {
-        s_src[j] = src;
-        s_dst[j] = dst;
-      }
+    if (!writes_table) {
+      const int dst = s_dst[lane];
+      __syncwarp();
+      if (again) s_dst[j] = dst;          // by copy
       if (lane == 0) s_n = ok ? __popc(agains) : 0;
     }
   }
   __syncthreads();
-  if (part == parts) {
+  if (writes_table) {
     int* ob = out + (size_t)b * K * cols;
-    for (int i = threadIdx.x; i < K * cols; i += 256) {
+    for (int i = threadIdx.x; i < K * cols; i += kCopyThreads) {
       const int r = i / cols, c = i % cols;
-      int v;
-      if (c < col) v = tb[s_par[r] * ldt + c];
-      else if (c == col && rem > 0) v = s_dst[r];
-      else v = tb[r * ldt + c];
-      ob[i] = v;
+      ob[i] = c < col ? tb[s_par[r] * ldt + c] : c == col && rem > 0 ? s_dst[r] : tb[r * ldt + c];
     }
     return;
   }
-  const int n16 = rem * row16;
-  for (int d = 0; d < s_n; ++d) {
+  for (int d = split; d < s_n; d += splits) {
     const uint4* src = pages + layer * ld_layer + s_src[d] * ld_page;
     uint4* dst = pages + layer * ld_layer + s_dst[d] * ld_page;
-    for (int i = part * 256 + threadIdx.x; i < n16; i += parts * 256) dst[i] = src[i];
+    uint4 v[kCopyVecs];
+#pragma unroll
+    for (int u = 0; u < kCopyVecs; ++u)
+      if (first + u * kCopyThreads < n16) v[u] = src[first + u * kCopyThreads];
+#pragma unroll
+    for (int u = 0; u < kCopyVecs; ++u)
+      if (first + u * kCopyThreads < n16) dst[first + u * kCopyThreads] = v[u];
   }
 }
 
@@ -289,23 +365,33 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> beam_select(const at:
   auto o_score = at::empty({B, K}, scores.options()), o_parent = at::empty({B, K}, iopt),
        o_token = at::empty({B, K}, iopt), o_done = at::empty({B, K}, scores.options().dtype(at::kBool));
   if (B == 0) return {o_score, o_parent, o_token, o_done};
-  const int nseg = (int)((V + kSelSeg - 1) / kSelSeg);
+  // 32 logits per thread where that gives two CTAs per SM, else 8: with few rows
+  // the latency of a segment counts, not its overhead (4 rows of 100,018: 12 us
+  // against 15 us)
+  const int64_t sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  const int per = B * K * ((V + 32 * kScanThreads - 1) / (32 * kScanThreads)) >= 2 * sms ? 32 : 8;
+  const int nseg = (int)((V + per * kScanThreads - 1) / (per * kScanThreads));
   auto work = at::empty({B * K * nseg * (1 + K) * 2}, scores.options());
   float2* stat = reinterpret_cast<float2*>(work.data_ptr());
-  uint2* cand = reinterpret_cast<uint2*>(stat + B * K * nseg);
+  uint64_t* cand = reinterpret_cast<uint64_t*>(stat + B * K * nseg);
   const dim3 grid(nseg, (unsigned)(B * K));
-  if (logits.scalar_type() == at::kFloat)
-    beam_scan_kernel<float><<<grid, kSelThreads, 0, st>>>(logits.data_ptr<float>(), logits.stride(0),
-                                                          logits.stride(1), (int)K, (int)V, (int)K, done, stat, cand);
-  else
-    beam_scan_kernel<bf16><<<grid, kSelThreads, 0, st>>>(reinterpret_cast<const bf16*>(logits.data_ptr()),
-                                                         logits.stride(0), logits.stride(1), (int)K, (int)V, (int)K,
-                                                         done, stat, cand);
+#define DSV3_SCAN(T_, PER_)                                                                                   \
+  beam_scan_kernel<T_, PER_><<<grid, kScanThreads, 0, st>>>(reinterpret_cast<const T_*>(logits.data_ptr()),  \
+                                                            logits.stride(0), logits.stride(1), (int)K,      \
+                                                            (int)V, done, stat, cand)
+  if (logits.scalar_type() == at::kFloat) {
+    if (per == 32) DSV3_SCAN(float, 32);
+    else DSV3_SCAN(float, 8);
+  } else {
+    if (per == 32) DSV3_SCAN(bf16, 32);
+    else DSV3_SCAN(bf16, 8);
+  }
+#undef DSV3_SCAN
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  beam_pick_kernel<<<(int)B, 256, 0, st>>>(stat, cand, scores.data_ptr<float>(), done, (int)K, (int)V, nseg, (int)eos,
-                                           o_score.data_ptr<float>(), o_parent.data_ptr<int>(),
-                                           o_token.data_ptr<int>(), o_done.data_ptr<bool>());
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  C10_CUDA_CHECK(launch_dependent(beam_pick_kernel, dim3((unsigned)B), kPickThreads, st, (const float2*)stat,
+                                  (const uint64_t*)cand, (const float*)scores.data_ptr<float>(), done, (int)K, (int)V,
+                                  nseg, (int)eos, o_score.data_ptr<float>(), o_parent.data_ptr<int>(),
+                                  o_token.data_ptr<int>(), o_done.data_ptr<bool>()));
   return {o_score, o_parent, o_token, o_done};
 }
 
@@ -334,12 +420,13 @@ at::Tensor beam_reorder(at::Tensor& pages, const at::Tensor& table, const at::Te
   auto out = at::empty({B * K, table.size(1)}, table.options());
   if (B == 0 || table.size(1) == 0) return out;
   const int row16 = (int)(width * es / 16);
-  const int parts = (int)((page * row16 + 1023) / 1024);
-  const dim3 grid(parts + 1, (unsigned)std::max<int64_t>(1, pages.size(0)), (unsigned)B);
-  beam_reorder_kernel<<<grid, 256, 0, at::cuda::getCurrentCUDAStream()>>>(
+  const int parts = (int)((page * row16 + kCopyThreads * kCopyVecs - 1) / (kCopyThreads * kCopyVecs));
+  const int splits = (int)std::max<int64_t>(1, K / 2);   // about K / e copies per group when parents are random
+  const dim3 grid(parts * splits + 1, (unsigned)std::max<int64_t>(1, pages.size(0)), (unsigned)B);
+  beam_reorder_kernel<<<grid, kCopyThreads, 0, at::cuda::getCurrentCUDAStream()>>>(
       reinterpret_cast<uint4*>(pages.data_ptr()), pages.stride(0) * es / 16, pages.stride(1) * es / 16, row16,
       (int)page, (int)pages.size(1), table.data_ptr<int>(), table.stride(0), (int)table.size(1),
-      parents.data_ptr<int>(), (int)K, lens.data_ptr<int>(), out.data_ptr<int>(), parts, status_ptr());
+      parents.data_ptr<int>(), (int)K, lens.data_ptr<int>(), out.data_ptr<int>(), parts, splits, status_ptr());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return out;
 }

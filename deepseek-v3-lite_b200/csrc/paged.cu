@@ -23,6 +23,7 @@
 #include <string>
 
 #include "common.cuh"
+#include "launch.h"
 #include "status.h"
 #include "tma_host.h"
 
@@ -194,8 +195,9 @@ at::Tensor paged_latent_attention(const at::Tensor& q, const at::Tensor& pages, 
   // fit in TMEM and the sequences fill it.
   const int64_t rows = (T * H + rg.B - 1) / rg.B;
   const int N = rows <= 16 ? 16 : rows <= 32 && T == rg.B ? 32 : rows <= 64 || R > 256 ? 64 : 128;
+  constexpr int KT = 64;
   PagedPlan pl;
-  TORCH_CHECK(paged_plan(N, (int)R, (int)D, pl), op, ": no shared-memory plan");
+  TORCH_CHECK(paged_plan(N, KT, (int)R, (int)D, pl), op, ": no shared-memory plan");
   auto work = at::empty({sms * (2 * N * (R + 2) + 4)}, q.options().dtype(at::kFloat));
   int4* rec = reinterpret_cast<int4*>(work.data_ptr<float>());
   float2* ml = reinterpret_cast<float2*>(rec + sms);
@@ -205,17 +207,17 @@ at::Tensor paged_latent_attention(const at::Tensor& q, const at::Tensor& pages, 
   const CUtensorMap tm_q = make_map(q.data_ptr(), 2, qd, qs, qb);
   const uint64_t kd[3] = {(uint64_t)D, (uint64_t)rg.page, (uint64_t)rg.pool};
   const uint64_t ks[2] = {(uint64_t)pages.stride(1) * 2, (uint64_t)pages.stride(0) * 2};
-  const uint32_t kb[3] = {64, (uint32_t)std::min(rg.page, 128), 1};
+  const uint32_t kb[3] = {64, (uint32_t)std::min(rg.page, KT), 1};
   const CUtensorMap tm_kv = make_map(pages.data_ptr(), 3, kd, ks, kb);
   auto st = at::cuda::getCurrentCUDAStream();
   const int64_t cuts = std::min<int64_t>(sms, T * H / N + rg.B);   // row tiles that can be cut, at most
   const bool few = cuts * 4 <= sms;
   bf16* o = reinterpret_cast<bf16*>(out.data_ptr());
-#define DSV3_PAGED(N_)                                                                                           \
+#define DSV3_PAGED(N_, KT_)                                                                                           \
   do {                                                                                                           \
-    C10_CUDA_CHECK(cudaFuncSetAttribute(paged_attention_tc_kernel<N_>,                                           \
+    C10_CUDA_CHECK(cudaFuncSetAttribute(paged_attention_tc_kernel<N_, KT_>,                                           \
                                         cudaFuncAttributeMaxDynamicSharedMemorySize, pl.smem));                  \
-    paged_attention_tc_kernel<N_><<<sms, kPaThreads, pl.smem, st>>>(                                             \
+    paged_attention_tc_kernel<N_, KT_><<<sms, kPaThreads, pl.smem, st>>>(                                             \
         tm_q, tm_kv, pl, rg, (int)T, (int)H, (int)R, (int)D, (float)(scale * 1.4426950408889634), 1, o, part, ml, \
         rec, status_ptr());                                                                                      \
     C10_CUDA_KERNEL_LAUNCH_CHECK();                                                                              \
@@ -224,10 +226,10 @@ at::Tensor paged_latent_attention(const at::Tensor& q, const at::Tensor& pages, 
                        : launch_dependent(paged_merge_kernel<N_, false>, dim3(sms, N_ / 8), 256, st,             \
                                           (const float*)part, (const float2*)ml, (const int4*)rec, sms, (int)R, o)); \
   } while (0)
-  if (N == 16) DSV3_PAGED(16);
-  else if (N == 32) DSV3_PAGED(32);
-  else if (N == 64) DSV3_PAGED(64);
-  else DSV3_PAGED(128);
+  if (N == 16) DSV3_PAGED(16, KT);
+  else if (N == 32) DSV3_PAGED(32, KT);
+  else if (N == 64) DSV3_PAGED(64, KT);
+  else DSV3_PAGED(128, KT);
 #undef DSV3_PAGED
   return out;
 }

@@ -35,57 +35,42 @@
 // which a second kernel merges in share order, so results do not depend on
 // timing.
 //
-// Warps: 0 TMA, 1 MMA (and TMEM), 2..9 softmax and epilogue.  Every wait is
+// Warps: 0 TMA, 1 first product (and TMEM), 2..9 softmax and epilogue, 10 second
+// product.  Every wait is
 // bounded; after one ran out the softmax warps go on without waiting, so that
 // they meet at their barriers, and the others stop.
 
-constexpr int kPaThreads = 320;
-constexpr int kPaChunk = 128 * 128;          // [128 keys x 64 columns] bf16, bytes
-constexpr int kPaPair = 2 * kPaChunk;
-constexpr int kPaMaxSlots = 8;
+constexpr int kPaThreads = 352;
+constexpr int kPaMaxSlots = 16;
 constexpr float kPaUnset = -1e30f;           // reference of a row that has seen no key
 constexpr float kPaLead = 12.f;              // first reference above the first key's score (log2)
 
 struct PagedPlan {
-  int N, LP, nch, tail;       // row tile, latent chunk pairs, chunks, 1 if there is a tail chunk
+  int LP, nch, tail;          // latent chunk pairs, chunks, 1 if there is a tail chunk
   int slots, tails;           // ring slots (pairs), tail slots
-  int alias;                  // P shares the (single) tail slot
-  int look;                   // S of the next tile is issued before PV of this one
   int off_q, off_p, off_t, off_misc, smem, tmem_cols;
 };
 
 // Shared memory of a plan: ring | tail slots | P | Q | misc, with as many ring
-// slots as fit.  P needs its own buffer unless even one whole key tile would
-// not fit next to it; then it takes the tail slot, which S has read by the time
-// P is written.
-inline bool paged_plan(int N, int R, int D, PagedPlan& p) {
-  p.N = N;
+// slots as fit; at least two key tiles' worth, so that one loads while the
+// other is in use.
+inline bool paged_plan(int N, int KT, int R, int D, PagedPlan& p) {
+  const int chunk = KT * 128;
   p.LP = (R + 127) / 128;
   p.nch = (D + 63) / 64;
   p.tail = D > 128 * p.LP ? 1 : 0;
-  const int limit = 232448;
-  const int q = p.nch * N * 128, P = (N + 63) / 64 * kPaChunk, misc = 12 * N + 1024 + 512;
-  for (int mode = 0; mode < 3; ++mode) {     // two tail slots, one, one shared with P
-    p.tails = p.tail ? (mode == 0 ? 2 : 1) : 0;
-    p.alias = p.tail && mode == 2;
-    if (p.alias && N > 64) continue;
-    const int fixed = q + (p.alias ? 0 : P) + p.tails * kPaChunk + misc;
-    const int fit = (limit - fixed) / kPaPair;
-    if (limit - fixed < 0 || fit < p.LP) continue;
-    p.slots = fit < kPaMaxSlots ? fit : kPaMaxSlots;
-    p.look = p.slots >= 2 * p.LP && (!p.tail || p.tails == 2);
-    if (mode == 0 && p.tail && !p.look) continue;   // the second tail slot only pays with lookahead
-    p.off_t = p.slots * kPaPair;
-    p.off_p = p.alias ? p.off_t : p.off_t + p.tails * kPaChunk;
-    p.off_q = (p.alias ? p.off_t + kPaChunk : p.off_p + P);
-    p.off_misc = p.off_q + q;
-    p.smem = p.off_misc + misc;
-    const int cols = (2 + p.LP) * N;
-    p.tmem_cols = 32;
-    while (p.tmem_cols < cols) p.tmem_cols *= 2;
-    return p.tmem_cols <= 512;
-  }
-  return false;
+  p.tails = p.tail ? 2 : 0;
+  const int q = p.nch * N * 128, P = (N + 63) / 64 * chunk, misc = 12 * N + 1024 + 512;
+  const int fit = (232448 - q - P - p.tails * chunk - misc) / (2 * chunk);
+  p.slots = fit < kPaMaxSlots ? fit : kPaMaxSlots;
+  p.off_t = p.slots * 2 * chunk;
+  p.off_p = p.off_t + p.tails * chunk;
+  p.off_q = p.off_p + P;
+  p.off_misc = p.off_q + q;
+  p.smem = p.off_misc + misc;
+  p.tmem_cols = 32;
+  while (p.tmem_cols < (2 + p.LP) * N) p.tmem_cols *= 2;
+  return p.slots >= 2 * p.LP && p.tmem_cols <= 512;
 }
 
 // sum_{i=0}^{n-1} floor((a i + b) / m) for a, b >= 0 (Euclid-like reduction, a
@@ -132,38 +117,44 @@ __device__ __forceinline__ PagedSeq paged_seq(const Ragged& r, int b, int H, int
   return s;
 }
 
+// A value that all lanes of the warp hold, marked as such for the compiler: loop
+// bounds and descriptors derived from it stay in uniform registers, and MMAs
+// under such control flow issue without moves or divergent branches (32 cycles
+// apiece against 67 to 200).
+__device__ __forceinline__ int warp_uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 // Key tiles of row tile rt: up to the position of its last row, at least one
 // (a row that sees nothing is still written).
-template <int N>
+template <int N, int KT>
 __device__ __forceinline__ int paged_key_tiles(const PagedSeq& s, int rt, int H) {
   const int last = min((rt + 1) * N, s.rows) - 1;
   const int keys = s.len - s.n + last / H + 1;
-  return max(1, (keys + 127) / 128);
+  return max(1, (keys + KT - 1) / KT);
 }
 
 // Key tiles of row tiles 0 .. k-1.
-template <int N>
+template <int N, int KT>
 __device__ __forceinline__ long long paged_tiles_before(const PagedSeq& s, int k, int H) {
   if (k <= 0) return 0;
   long long ans = 0;
   int full = k;
   if (k == s.tiles) {         // the last row tile may be short
     full = k - 1;
-    ans = paged_key_tiles<N>(s, k - 1, H);
+    ans = paged_key_tiles<N, KT>(s, k - 1, H);
   }
   // row tile i ends at row x = (i + 1) N - 1, at position p = len - n + x / H:
-  // p / 128 + 1 = ((len - n) H + x) / (128 H) + 1 tiles, one where p < 0
+  // p / KT + 1 = ((len - n) H + x) / (KT H) + 1 tiles, one where p < 0
   const long long c = (long long)(s.len - s.n) * H + N - 1;
   int first = 0;
   if (c < 0) first = (int)min((long long)full, (-c + N - 1) / N);
   const long long b = c + (long long)first * N;
   if (b + (long long)full * N < (1ll << 31))
-    return ans + full + floor_sum<uint32_t>(full - first, 128u * H, N, (uint32_t)b);
-  return ans + full + floor_sum<long long>(full - first, 128ll * H, N, b);
+    return ans + full + floor_sum<uint32_t>(full - first, (uint32_t)KT * H, N, (uint32_t)b);
+  return ans + full + floor_sum<long long>(full - first, (long long)KT * H, N, b);
 }
 
 // A CTA's share as a walk over items: (sequence, row tile, key tiles t0 .. t1).
-template <int N>
+template <int N, int KT>
 struct PagedWalk {
   const Ragged& r;
   int H, total;
@@ -173,10 +164,18 @@ struct PagedWalk {
   __device__ __forceinline__ PagedWalk(const Ragged& r_, int H_, int total_, int count, int b0, int rt0, int tile0)
       : r(r_), H(H_), total(total_), left(count), b(b0), rt(rt0), t0(tile0) {
     if (left > 0) {
-      s = paged_seq<N>(r, b, H, total);
-      nt = paged_key_tiles<N>(s, rt, H);
+      load();
+      nt = paged_key_tiles<N, KT>(s, rt, H);
       t1 = min(nt, t0 + left);
     }
+  }
+  __device__ __forceinline__ void load() {
+    s = paged_seq<N>(r, b, H, total);
+    s.tok0 = warp_uniform(s.tok0);
+    s.n = warp_uniform(s.n);
+    s.len = warp_uniform(s.len);
+    s.rows = s.n * H;
+    s.tiles = (s.rows + N - 1) / N;
   }
   __device__ __forceinline__ bool ok() const { return left > 0; }
   __device__ __forceinline__ void next() {
@@ -190,10 +189,10 @@ struct PagedWalk {
           left = 0;
           return;
         }
-        s = paged_seq<N>(r, b, H, total);
+        load();
       } while (s.tiles == 0);
     }
-    nt = paged_key_tiles<N>(s, rt, H);
+    nt = paged_key_tiles<N, KT>(s, rt, H);
     t1 = min(nt, left);
   }
 };
@@ -217,6 +216,36 @@ __device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, uint32_t (&r)[NC]) 
 #pragma unroll
     for (int i = 0; i < NC; i += 16) tmem_ld16(taddr + i, *reinterpret_cast<uint32_t(*)[16]>(&r[i]));
   }
+}
+// Lanes 0..15 of the warp's quarter: threads 0..15 get W columns at taddr,
+// threads 16..31 those SPLIT columns further of the same lanes.
+template <int SPLIT, int W>
+__device__ __forceinline__ void tmem_ld_half(uint32_t taddr, uint32_t* r) {
+  if constexpr (W == 4) {
+    asm volatile("tcgen05.ld.sync.aligned.16x32bx2.x4.b32 {%0, %1, %2, %3}, [%4], %5;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(taddr), "n"(SPLIT));
+  } else if constexpr (W == 8) {
+    asm volatile("tcgen05.ld.sync.aligned.16x32bx2.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8], %9;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr), "n"(SPLIT));
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; i += 16)
+      asm volatile(
+          "tcgen05.ld.sync.aligned.16x32bx2.x16.b32 "
+          "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16], %17;"
+          : "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]),
+            "=r"(r[i + 7]), "=r"(r[i + 8]), "=r"(r[i + 9]), "=r"(r[i + 10]), "=r"(r[i + 11]), "=r"(r[i + 12]),
+            "=r"(r[i + 13]), "=r"(r[i + 14]), "=r"(r[i + 15])
+          : "r"(taddr + i), "n"(SPLIT));
+  }
+}
+// W columns of S^T of this thread's key, at column c of its group.
+template <int KT, int NC, int W>
+__device__ __forceinline__ void ld_scores(uint32_t taddr, uint32_t (&r)[W]) {
+  if constexpr (KT == 64) tmem_ld_half<NC, W>(taddr, r);
+  else tmem_ld_cols<W>(taddr, r);
 }
 
 // Barrier of the 128 threads of one column half, with the OR of a predicate.
@@ -253,7 +282,7 @@ struct PagedStart {
   int b, rt, tile, found;
 };
 
-template <int N>
+template <int N, int KT>
 __device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, int min_share, PagedStart* out, int* scan, unsigned int* status) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int NW = kPaThreads / 32;
@@ -271,7 +300,7 @@ __device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, in
         t = 0;
         if (b < r.B) {
           s = paged_seq<N>(r, b, H, total);
-          t = (int)paged_tiles_before<N>(s, s.tiles, H);
+          t = (int)paged_tiles_before<N, KT>(s, s.tiles, H);
           if (round == 0 && blockIdx.x == 0) {
             const int c0 = __ldg(r.cu + b), c1 = __ldg(r.cu + b + 1);
             if (__ldg(r.lens + b) > r.cols * r.page || c1 > total || c1 < c0 || (b == 0 && c0 != 0) ||
@@ -330,8 +359,8 @@ __device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, in
       const int step = (hi - lo + kPaThreads - 1) / kPaThreads, k = lo + tid * step;
       const int k1 = min(k + step, hi);
       if (k < hi) {
-        const long long at = paged_tiles_before<N>(s, k, H);
-        if (at <= local && (k1 == s.tiles || local < paged_tiles_before<N>(s, k1, H))) {
+        const long long at = paged_tiles_before<N, KT>(s, k, H);
+        if (at <= local && (k1 == s.tiles || local < paged_tiles_before<N, KT>(s, k1, H))) {
           out->rt = k;
           out->tile = (int)(local - at);
         }
@@ -344,12 +373,12 @@ __device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, in
   }
 }
 
-// Combines W values per lane over the 32 lanes of a warp, column by column: W
-// / 2 exchanges, then W / 4 ..., since a lane keeps only half of its columns at
-// each step.  Lane i ends with column i * W / 32.
-template <int W, typename Op>
+// Combines W values per lane over groups of L lanes, column by column: W / 2
+// exchanges, then W / 4 ..., since a lane keeps only half of its columns at each
+// step.  Lane i of a group ends with column i * W / L.
+template <int W, int L, typename Op>
 __device__ __forceinline__ float fold_columns(float (&v)[W], int lane, Op op) {
-  int o = 16;
+  int o = L / 2;
 #pragma unroll
   for (int w = W; w > 1; w >>= 1, o >>= 1) {
     const bool up = lane & o;
@@ -387,6 +416,37 @@ __device__ __forceinline__ void commit_lead(uint32_t leader, uint64_t* bar) {
       "r"(smem_u32(bar))
       : "memory");
 }
+// The issuing lane.  It has to come from elect.sync: under `lane == 0` the
+// compiler wraps each MMA in a divergent branch (90 to 200 cycles apiece).
+// The TMA loads and barrier arrivals of the producer are issued the same way.
+__device__ __forceinline__ void expect_lead(uint32_t leader, uint64_t* bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %0, 0;\n\t"
+      "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%1], %2;\n\t}" ::"r"(leader),
+      "r"(smem_u32(bar)), "r"(bytes)
+      : "memory");
+}
+__device__ __forceinline__ void tma_lead_2d(uint32_t leader, uint32_t dst, const void* desc, uint64_t* bar, int c0,
+                                            int c1) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %0, 0;\n\t"
+      "@q cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%1], [%2, {%4, %5}], [%3];\n\t}" ::
+          "r"(leader),
+      "r"(dst), "l"(desc), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void tma_lead_3d(uint32_t leader, uint32_t dst, const void* desc, uint64_t* bar, int c0,
+                                            int c1, int c2) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %0, 0;\n\t"
+      "@q cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%1], [%2, {%4, %5, %6}], "
+      "[%3];\n\t}" ::"r"(leader),
+      "r"(dst), "l"(desc), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
 __device__ __forceinline__ uint32_t elect_lead() {
   uint32_t r;
   asm volatile(
@@ -397,11 +457,40 @@ __device__ __forceinline__ uint32_t elect_lead() {
   return r;
 }
 
+// mbar_wait_bounded with a hint to sleep up to 20 us per try: some 300 threads
+// wait at any time here, and their polling slowed the issuing warps down.
+__device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, unsigned int* status,
+                                        unsigned int code) {
+  uint64_t t0 = 0;
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
+        : "memory");
+    if (ok) return true;
+    if (*abort_flag) return false;
+    const uint64_t now = globaltimer_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > DSV3_WAIT_BUDGET_NS) {
+      record_error(status, code);
+      *abort_flag = 1;
+      return false;
+    }
+  }
+}
+
 // Low words of the shared-memory descriptors (128-byte swizzle, 1024 bytes
 // between groups of eight rows) and the high word that both share.
 constexpr uint32_t kPaDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
 __device__ __forceinline__ uint32_t desc_k(uint32_t addr) { return (addr >> 4) | (1u << 16); }
-__device__ __forceinline__ uint32_t desc_mn(uint32_t addr) { return (addr >> 4) | ((uint32_t)(kPaChunk >> 4) << 16); }
+template <int CHUNK>
+__device__ __forceinline__ uint32_t desc_mn(uint32_t addr) {
+  return (addr >> 4) | ((uint32_t)(CHUNK >> 4) << 16);
+}
 
 // Position in a ring of slots.
 struct Ring {
@@ -416,12 +505,13 @@ struct Ring {
   }
 };
 
-template <int N>
+template <int N, int KT>
 __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
-    const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_kv, PagedPlan pl, Ragged rg,
+    const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ PagedPlan pl,
+    const __grid_constant__ Ragged rg,
     int total, int H, int R, int D, float scale_log2, int min_share, bf16* __restrict__ out,
     float* __restrict__ part_o, float2* __restrict__ part_ml, int4* __restrict__ rec, unsigned int* status) {
-  constexpr int NC = N / 2;
+  constexpr int CHUNK = KT * 128, PAIR = 2 * CHUNK;  // [KT keys x 64 columns], two of them (bytes)
   extern __shared__ __align__(1024) uint8_t smem[];
   float* mref = reinterpret_cast<float*>(smem + pl.off_misc);            // [N]
   int* lim = reinterpret_cast<int*>(mref + N);                           // [N] keys that a row sees
@@ -437,8 +527,9 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
   uint64_t* p_ready = s_full + 2;
   uint64_t* pv_done = p_ready + 1;
   uint64_t* o_free = pv_done + 1;
-  uint64_t* drain = o_free + 1;
-  PagedStart* start = reinterpret_cast<PagedStart*>(drain + 1);
+  uint64_t* s_free = o_free + 1;      // [2]
+  uint64_t* drain = s_free + 2;       // [2]
+  PagedStart* start = reinterpret_cast<PagedStart*>(drain + 2);
   int* scan = reinterpret_cast<int*>(start + 1);             // [kPaThreads / 32]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(scan + kPaThreads / 32);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -460,7 +551,10 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
     mbar_init(p_ready, 8);
     mbar_init(pv_done, 1);
     mbar_init(o_free, 8);
-    mbar_init(drain, 1);
+    mbar_init(&s_free[0], 8);
+    mbar_init(&s_free[1], 8);
+    mbar_init(&drain[0], 1);
+    mbar_init(&drain[1], 1);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tm_q);
@@ -471,34 +565,33 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
     tmem_relinquish();
   }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  paged_find<N>(rg, H, total, min_share, start, scan, status);
+  paged_find<N, KT>(rg, H, total, min_share, start, scan, status);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  const int count = start->count;
+  const uint32_t tmem = warp_uniform(*tmem_slot);
+  const int count = warp_uniform(start->count), b_0 = warp_uniform(start->b), rt_0 = warp_uniform(start->rt),
+            tile_0 = warp_uniform(start->tile);
   const uint32_t smem0 = smem_u32(smem);
-  const int boxes = rg.page >= 128 ? 1 : 128 / rg.page;        // TMA boxes per chunk
+  const int boxes = rg.page >= KT ? 1 : KT / rg.page;        // TMA boxes per chunk
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
+    const uint32_t lead = elect_lead();
     Ring pr(pl.slots), tr(pl.tail ? pl.tails : 1);
     uint32_t pu = 0, tu = 0, items = 0;      // pair uses, tail uses
-    bool ok = count > 0;
-    for (PagedWalk<N> w(rg, H, total, ok ? count : 0, start->b, start->rt, start->tile); w.ok() && ok; w.next(), ++items) {
-      if (lane == 0) {
-        ok = mbar_wait_bounded(q_empty, (items & 1u) ^ 1u, abort_flag, status, DSV3_ERR_WAIT_EMPTY);
-        if (ok) {
-          mbar_arrive_expect_tx(q_full, pl.nch * N * 128);
-          const int row = w.s.tok0 * H + w.rt * N;
-          for (int c = 0; c < pl.nch; ++c) tma_load_2d(smem + pl.off_q + c * N * 128, &tm_q, q_full, 64 * c, row);
-        }
-      }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
+    bool ok = true;
+    for (PagedWalk<N, KT> w(rg, H, total, count, b_0, rt_0, tile_0); w.ok() && ok; w.next()) {
+      ok = pa_wait(q_empty, (items & 1u) ^ 1u, abort_flag, status, DSV3_ERR_WAIT_EMPTY);
+      if (!ok) break;
+      ++items;
+      expect_lead(lead, q_full, pl.nch * N * 128);
+      const int qrow = w.s.tok0 * H + w.rt * N;
+      for (int c = 0; c < pl.nch; ++c) tma_lead_2d(lead, smem0 + pl.off_q + c * N * 128, &tm_q, q_full, 64 * c, qrow);
       for (int t = w.t0; t < w.t1 && ok; ++t) {
         // page of this lane's box; one outside the pool reads as zeros
         int pg = rg.pool;
-        const int key = t * 128 + lane * (128 / boxes);
+        const int key = t * KT + lane * (KT / boxes);
         if (lane < boxes && key < w.s.len) {
           pg = rg.table[w.b * rg.ldt + key / rg.page];
           if (pg < 0 || pg >= rg.pool) {
@@ -506,36 +599,32 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
             pg = rg.pool;
           }
         }
-        const int row = key & (rg.page - 1);
-        const int dst = lane * (128 / boxes) * 128;
-        for (int m = 0; m <= pl.LP && ok; ++m) {
-          if (m == pl.LP && !pl.tail) break;
+        const int row = t * KT & (rg.page - 1);
+        for (int m = 0; m < pl.LP + pl.tail; ++m) {
           const bool is_tail = m == pl.LP;
           const int c0 = 2 * m, nc = is_tail ? 1 : min(2, pl.nch - c0);
           const int slot = is_tail ? tr.slot : pr.slot;
-          const uint32_t ph = is_tail ? tr.phase : pr.phase;
           uint64_t* full = is_tail ? &tail_full[slot] : &pair_full[slot];
-          uint64_t* empty = is_tail ? &tail_empty[slot] : &pair_empty[slot];
-          uint8_t* at = smem + (is_tail ? pl.off_t + slot * kPaChunk : slot * kPaPair);
-          if (lane == 0) {
-            ok = mbar_wait_bounded(empty, ph ^ 1u, abort_flag, status, DSV3_ERR_WAIT_EMPTY);
-            if (ok) mbar_arrive_expect_tx(full, nc * kPaChunk);
+          const uint32_t at = smem0 + (is_tail ? pl.off_t + slot * CHUNK : slot * PAIR);
+          ok = pa_wait(is_tail ? &tail_empty[slot] : &pair_empty[slot], (is_tail ? tr.phase : pr.phase) ^ 1u, abort_flag,
+                       status, DSV3_ERR_WAIT_EMPTY);
+          if (!ok) break;
+          expect_lead(lead, full, nc * CHUNK);
+          for (int i = 0; i < boxes; ++i) {
+            const int p = __shfl_sync(0xffffffffu, pg, i);
+            const uint32_t dst = at + i * (KT / boxes) * 128;
+            tma_lead_3d(lead, dst, &tm_kv, full, 64 * c0, row, p);
+            if (nc > 1) tma_lead_3d(lead, dst + CHUNK, &tm_kv, full, 64 * c0 + 64, row, p);
           }
-          ok = __shfl_sync(0xffffffffu, ok, 0);
-          if (ok && lane < boxes)
-            for (int c = 0; c < nc; ++c) tma_load_3d(at + c * kPaChunk + dst, &tm_kv, full, 64 * (c0 + c), row, pg);
-          if (ok) {
-            if (is_tail) {
-              tr.next();
-              ++tu;
-            } else {
-              pr.next();
-              ++pu;
-            }
+          if (is_tail) {
+            tr.next();
+            ++tu;
+          } else {
+            pr.next();
+            ++pu;
           }
         }
       }
-      if (!ok) break;
     }
     // every issued copy lands before the CTA may exit
     if (lane == 0) {
@@ -546,92 +635,60 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
       if (items > 0) mbar_wait_bounded(q_full, (items - 1) & 1u, nullptr, status, DSV3_ERR_WAIT_FULL);
     }
   } else if (warp == 1) {
-    // ---------------------------------------------------------- MMA issuer
+    // --------------------------------------------------------- S^T = K Q^T
     if (count > 0) {
-      constexpr uint32_t I_S = idesc_bf16_f32(128, N, 0, 0);     // S^T = K Q^T
-      constexpr uint32_t I_O = idesc_bf16_f32(128, N, 1, 1);     // O^T += V^T P^T, both read MN-major
+      constexpr uint32_t I_S = idesc_bf16_f32(KT, N, 0, 0);
       const uint32_t lead = elect_lead();
-      PagedWalk<N> ws(rg, H, total, count, start->b, start->rt, start->tile);   // walk of S
-      PagedWalk<N> wp(rg, H, total, count, start->b, start->rt, start->tile);   // walk of PV
-      Ring sr(pl.slots), tr(pl.tail ? pl.tails : 1), vr(pl.slots);
-      int ts = ws.t0, tp = wp.t0;
-      uint32_t gs = 0, gp = 0, s_items = 0, p_items = 0;
+      Ring sr(pl.slots), tr(pl.tail ? pl.tails : 1);
+      uint32_t g = 0, items = 0;
       bool ok = true, issued = false;
-      const uint32_t p_lo = desc_mn(smem0 + pl.off_p);
-      // S^T of the next tile in order
-      auto issue_s = [&]() {
-        if (ts == ws.t0) {
-          if (!mbar_wait_bounded(q_full, s_items & 1u, abort_flag, status, DSV3_ERR_WAIT_FULL)) return false;
-        }
-        const uint32_t d = tmem + (gs & 1u) * N;
-        uint32_t acc = 0;
-        uint32_t q_lo = desc_k(smem0 + pl.off_q);
-        for (int m = 0; m < pl.LP + pl.tail; ++m) {
-          const bool is_tail = m == pl.LP;
-          const int slot = is_tail ? tr.slot : sr.slot;
-          if (!mbar_wait_bounded(is_tail ? &tail_full[slot] : &pair_full[slot], is_tail ? tr.phase : sr.phase,
-                                 abort_flag, status, DSV3_ERR_WAIT_FULL))
-            return false;
-          tc_fence_after();
-          uint32_t a_lo = desc_k(smem0 + (is_tail ? pl.off_t + slot * kPaChunk : slot * kPaPair));
-          int left = D - 128 * m;               // columns of this pair that hold data
-          for (int c = 0; c < 2 && left > 0; ++c) {
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              if (16 * kk < left) {
-                umma_lead(lead, d, a_lo + 2 * kk, q_lo + 2 * kk, kPaDescHi, I_S, acc);
-                acc = 1;
-              }
-            a_lo += kPaChunk >> 4;
-            q_lo += N * 128 >> 4;
-            left -= 64;
+      for (PagedWalk<N, KT> w(rg, H, total, count, b_0, rt_0, tile_0); w.ok() && ok; w.next(), ++items) {
+        ok = pa_wait(q_full, items & 1u, abort_flag, status, DSV3_ERR_WAIT_FULL);
+        for (int t = w.t0; t < w.t1 && ok; ++t, ++g) {
+          // two S^T buffers: this one's last tile has been read
+          if (g > 1 && !pa_wait(&s_free[g & 1u], ((g >> 1) & 1u) ^ 1u, abort_flag, status, DSV3_ERR_WAIT_TMEM)) {
+            ok = false;
+            break;
           }
-          issued = true;
-          if (is_tail) {
-            if (!pl.alias) commit_lead(lead, &tail_empty[slot]);
-            tr.next();
-          } else {
-            sr.next();
-          }
-        }
-        commit_lead(lead, &s_full[gs & 1u]);
-        ++gs;
-        if (++ts >= ws.t1) {
-          commit_lead(lead, q_empty);
-          ++s_items;
-          ws.next();
-          ts = ws.t0;
-        }
-        return true;
-      };
-      ok = issue_s();
-      while (ok && wp.ok()) {
-        if (pl.look && ws.ok()) ok = issue_s();
-        if (!ok) break;
-        if (!mbar_wait_bounded(p_ready, gp & 1u, abort_flag, status, DSV3_ERR_WAIT_FULL)) break;
-        const bool first = tp == wp.t0;
-        if (first && p_items > 0 &&
-            !mbar_wait_bounded(o_free, (p_items - 1) & 1u, abort_flag, status, DSV3_ERR_WAIT_TMEM))
-          break;
-        tc_fence_after();
-        for (int m = 0; m < pl.LP; ++m) {
-          const uint32_t v_lo = desc_mn(smem0 + vr.slot * kPaPair), d = tmem + (2 + m) * N;
-          umma_lead(lead, d, v_lo, p_lo, kPaDescHi, I_O, first ? 0u : 1u);
+          const uint32_t d = tmem + (g & 1u) * N;
+          uint32_t acc = 0, q_lo = desc_k(smem0 + pl.off_q);
+          for (int m = 0; m < pl.LP + pl.tail; ++m) {
+            const bool is_tail = m == pl.LP;
+            const int slot = is_tail ? tr.slot : sr.slot;
+            if (!pa_wait(is_tail ? &tail_full[slot] : &pair_full[slot], is_tail ? tr.phase : sr.phase, abort_flag,
+                         status, DSV3_ERR_WAIT_FULL)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            uint32_t a_lo = desc_k(smem0 + (is_tail ? pl.off_t + slot * CHUNK : slot * PAIR));
+            // 64-column chunks of this pair: whole ones as four MMAs, what is left
+            // of the row as its steps of 16
+            const int left = min(128, D - 128 * m);
+            for (int c = 0; c < left / 64; ++c) {
+              umma_lead(lead, d, a_lo, q_lo, kPaDescHi, I_S, acc);
 #pragma unroll
-          for (int kk = 1; kk < 8; ++kk) umma_lead(lead, d, v_lo + 128 * kk, p_lo + 128 * kk, kPaDescHi, I_O, 1u);
-          commit_lead(lead, &pair_empty[vr.slot]);
-          vr.next();
+              for (int kk = 1; kk < 4; ++kk) umma_lead(lead, d, a_lo + 2 * kk, q_lo + 2 * kk, kPaDescHi, I_S, 1u);
+              acc = 1;
+              a_lo += CHUNK >> 4;
+              q_lo += N * 128 >> 4;
+            }
+#pragma unroll 1
+            for (int k = 0; k < left % 64; k += 16) {
+              umma_lead(lead, d, a_lo + k / 8, q_lo + k / 8, kPaDescHi, I_S, acc);
+              acc = 1;
+            }
+            issued = true;
+            if (is_tail) {
+              commit_lead(lead, &tail_empty[slot]);
+              tr.next();
+            } else {
+              sr.next();
+            }
+          }
+          if (ok) commit_lead(lead, &s_full[g & 1u]);
         }
-        if (pl.alias) commit_lead(lead, &tail_empty[0]);
-        commit_lead(lead, pv_done);
-        issued = true;
-        ++gp;
-        if (++tp >= wp.t1) {
-          ++p_items;
-          wp.next();
-          tp = wp.t0;
-        }
-        if (!pl.look && ws.ok()) ok = issue_s();
+        if (ok) commit_lead(lead, q_empty);
       }
       if (issued) {   // no MMA may still write TMEM when it is freed
         commit_lead(lead, drain);
@@ -639,25 +696,70 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
       }
       __syncwarp();
     }
+  } else if (warp == 10) {
+    // ------------------------------------------------------ O^T += V^T P^T
+    // A warp of its own: S^T of a later tile and PV of this one become ready in
+    // either order, and neither waits behind the other.
+    if (count > 0) {
+      constexpr uint32_t I_O = idesc_bf16_f32(128, N, 1, 1);     // both read MN-major
+      const uint32_t lead = elect_lead();
+      Ring vr(pl.slots);
+      const uint32_t p_lo = desc_mn<CHUNK>(smem0 + pl.off_p);
+      uint32_t g = 0, items = 0;
+      bool ok = true, issued = false;
+      for (PagedWalk<N, KT> w(rg, H, total, count, b_0, rt_0, tile_0); w.ok() && ok; w.next(), ++items) {
+        for (int t = w.t0; t < w.t1 && ok; ++t, ++g) {
+          ok = pa_wait(p_ready, g & 1u, abort_flag, status, DSV3_ERR_WAIT_FULL);
+          // the last item's O^T has been read out
+          if (ok && t == w.t0 && items > 0)
+            ok = pa_wait(o_free, (items - 1) & 1u, abort_flag, status, DSV3_ERR_WAIT_TMEM);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t acc = t > w.t0;
+          for (int m = 0; m < pl.LP; ++m) {
+            const uint32_t v_lo = desc_mn<CHUNK>(smem0 + vr.slot * PAIR), d = tmem + (2 + m) * N;
+            umma_lead(lead, d, v_lo, p_lo, kPaDescHi, I_O, acc);
+#pragma unroll
+            for (int kk = 1; kk < KT / 16; ++kk)
+              umma_lead(lead, d, v_lo + 128 * kk, p_lo + 128 * kk, kPaDescHi, I_O, 1u);
+            commit_lead(lead, &pair_empty[vr.slot]);
+            vr.next();
+          }
+          commit_lead(lead, pv_done);
+          issued = true;
+        }
+      }
+      if (issued) {
+        commit_lead(lead, drain + 1);
+        mbar_wait_bounded(drain + 1, 0, nullptr, status, DSV3_ERR_WAIT_TMEM);
+      }
+      __syncwarp();
+    }
   } else {
     // ---------------------------------------------------- softmax / epilogue
     const int half = (warp - 2) >> 2;              // columns half * NC ..
     const int quarter = warp & 3;                  // TMEM lanes 32 * quarter ..
-    const int key = quarter * 32 + lane;           // key of S^T, latent column of O^T
+    // A key tile of 64 fills 16 TMEM lanes of each quarter; the two half warps
+    // then take different columns of the same 16 keys.
+    constexpr int NC = KT == 64 ? N / 4 : N / 2;   // score columns of a thread
+    constexpr int L = KT == 64 ? 16 : 32;          // lanes that hold different keys
+    constexpr int NH = N / 2;                      // columns of a half
+    const int group = KT == 64 ? lane >> 4 : 0;
+    const int key = quarter * L + (lane & (L - 1));
     const int ht = (warp - 2 - 4 * half) * 32 + lane;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-    const int col0 = half * NC;
+    const int col0 = half * NH + group * NC;
     float* myred = red + half * 128;               // [32][4]
     float4* mref4 = reinterpret_cast<float4*>(mref + col0);
     const int4* lim4 = reinterpret_cast<const int4*>(lim + col0);
     uint32_t g = 0;
     int4 my_rec = make_int4(-1, 0, 0, 0);
-    for (PagedWalk<N> w(rg, H, total, count, start->b, start->rt, start->tile); w.ok(); w.next()) {
+    for (PagedWalk<N, KT> w(rg, H, total, count, b_0, rt_0, tile_0); w.ok(); w.next()) {
       const int base = w.s.len - w.s.n;
       const int nr = min(N, w.s.rows - w.rt * N);
       half_sync(half);                             // the last item's references are read
-      if (ht < NC) {
-        const int n = col0 + ht;
+      if (ht < NH) {
+        const int n = half * NH + ht;
         reinterpret_cast<uint32_t*>(corr)[n] = 0u;
         lim[n] = n < nr ? base + (w.rt * N + n) / H + 1 : 0;
       }
@@ -667,13 +769,13 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
 #pragma unroll
       for (int c = 0; c < NC; ++c) l[c] = 0.f;
       for (int t = w.t0; t < w.t1; ++t, ++g) {
-        mbar_wait_bounded(&s_full[g & 1u], (g >> 1) & 1u, abort_flag, status, DSV3_ERR_WAIT_TMEM);
+        pa_wait(&s_full[g & 1u], (g >> 1) & 1u, abort_flag, status, DSV3_ERR_WAIT_TMEM);
         tc_fence_after();
         uint32_t sr[NC];
-        tmem_ld_cols<NC>(tmem + lane_base + (g & 1u) * N + col0, sr);
+        ld_scores<KT, NC, NC>(tmem + lane_base + (g & 1u) * N + half * NH, sr);
         tmem_ld_wait();
-        const int pos = t * 128 + key;
-        if (t * 128 + 128 > seen_by_all) {
+        const int pos = t * KT + key;
+        if (t * KT + KT > seen_by_all) {
 #pragma unroll
           for (int c = 0; c < NC; c += 4) {
             const int4 k4 = lim4[c / 4];
@@ -727,21 +829,22 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
           for (int c0 = 0; c0 < NC; c0 += W) {
             uint32_t u[W];
             float v[W];
-            tmem_ld_cols<W>(tmem + lane_base + (g & 1u) * N + col0 + c0, u);
+            ld_scores<KT, NC, W>(tmem + lane_base + (g & 1u) * N + half * NH + c0, u);
             tmem_ld_wait();
 #pragma unroll
             for (int c = 0; c < W; ++c)
               v[c] = pos < lim[col0 + c0 + c] ? __uint_as_float(u[c]) * scale_log2 : -INFINITY;
-            const float top = fold_columns<W>(v, lane, [](float x, float y) { return fmaxf(x, y); });
-            if (lane % (32 / W) == 0)
-              atomicMax(reinterpret_cast<unsigned int*>(corr) + col0 + c0 + lane * W / 32, float_key(top));
+            const float top = fold_columns<W, L>(v, lane, [](float x, float y) { return fmaxf(x, y); });
+            if (lane % (L / W) == 0)
+              atomicMax(reinterpret_cast<unsigned int*>(corr) + col0 + c0 + (lane & (L - 1)) * W / L, float_key(top));
           }
           half_sync(half);
-          if (ht < NC) {
-            const float old = mref[col0 + ht], top = float_unkey(reinterpret_cast<uint32_t*>(corr)[col0 + ht]);
+          if (ht < NH) {
+            const int n = half * NH + ht;
+            const float old = mref[n], top = float_unkey(reinterpret_cast<uint32_t*>(corr)[n]);
             const float now = fmaxf(old, top);
-            mref[col0 + ht] = now;
-            corr[col0 + ht] = ex2_approx(old - now);
+            mref[n] = now;
+            corr[n] = ex2_approx(old - now);
           }
           half_sync(half);
 #pragma unroll
@@ -753,38 +856,45 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
             l[c + 3] *= f.w;
           }
           if (t > w.t0) {   // the first tile of an item overwrites O^T
-            mbar_wait_bounded(pv_done, (g - 1) & 1u, abort_flag, status, DSV3_ERR_WAIT_TMEM);
+            pa_wait(pv_done, (g - 1) & 1u, abort_flag, status, DSV3_ERR_WAIT_TMEM);
             tc_fence_after();
 #pragma unroll 1
-            for (int i = 0; i < pl.LP * (NC / 8); ++i) {
-              const int m = i / (NC / 8), c = i % (NC / 8) * 8;
+            for (int i = 0; i < pl.LP * (NH / 8); ++i) {
+              const int m = i / (NH / 8), c = half * NH + i % (NH / 8) * 8;
               uint32_t o[8];
-              tmem_ld8(tmem + lane_base + (2 + m) * N + col0 + c, o);
+              tmem_ld8(tmem + lane_base + (2 + m) * N + c, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr[col0 + c + j]);
-              tmem_st8(tmem + lane_base + (2 + m) * N + col0 + c, o);
+              for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr[c + j]);
+              tmem_st8(tmem + lane_base + (2 + m) * N + c, o);
             }
             tmem_st_wait();
           }
           half_sync(half);
-          if (ht < NC) reinterpret_cast<uint32_t*>(corr)[col0 + ht] = 0u;
+          if (ht < NH) reinterpret_cast<uint32_t*>(corr)[half * NH + ht] = 0u;
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[g & 1u]);
         // P and O^T of the previous tile are no longer in use by the tensor core
-        if (g > 0) mbar_wait_bounded(pv_done, (g - 1) & 1u, abort_flag, status, DSV3_ERR_WAIT_TMEM);
+        if (g > 0) pa_wait(pv_done, (g - 1) & 1u, abort_flag, status, DSV3_ERR_WAIT_TMEM);
         uint8_t* prow = smem + pl.off_p + key * 128;
+        if constexpr (NC == 4) {
+          *reinterpret_cast<uint2*>(prow + (((col0 >> 3) ^ (key & 7)) << 4) + (col0 & 4) * 2) = make_uint2(pk[0], pk[1]);
+        } else {
 #pragma unroll
-        for (int c = 0; c < NC; c += 8) {
-          const int n = col0 + c;
-          *reinterpret_cast<uint4*>(prow + (n >> 6) * kPaChunk + ((((n & 63) >> 3) ^ (key & 7)) << 4)) =
-              make_uint4(pk[c / 2], pk[c / 2 + 1], pk[c / 2 + 2], pk[c / 2 + 3]);
+          for (int c = 0; c < NC; c += 8) {
+            const int n = col0 + c;
+            *reinterpret_cast<uint4*>(prow + (n >> 6) * CHUNK + ((((n & 63) >> 3) ^ (key & 7)) << 4)) =
+                make_uint4(pk[c / 2], pk[c / 2 + 1], pk[c / 2 + 2], pk[c / 2 + 3]);
+          }
         }
         // rows of the pages past the cached length hold anything: zero them, so
         // that their zero weights do not meet an infinity or NaN
-        if (t * 128 + 128 > w.s.len && pos >= w.s.len) {
-          for (int c = half; c < 2 * pl.LP; c += 2) {
+        if (t * KT + KT > w.s.len && pos >= w.s.len) {
+          for (int c = KT == 64 ? half * 2 + group : half; c < 2 * pl.LP; c += KT == 64 ? 4 : 2) {
             const int slot = (g * pl.LP + (c >> 1)) % pl.slots;
-            uint4* z = reinterpret_cast<uint4*>(smem + slot * kPaPair + (c & 1) * kPaChunk + key * 128);
+            uint4* z = reinterpret_cast<uint4*>(smem + slot * PAIR + (c & 1) * CHUNK + key * 128);
 #pragma unroll
             for (int i = 0; i < 8; ++i) z[(i + lane) & 7] = make_uint4(0, 0, 0, 0);   // spread over the banks
           }
@@ -801,7 +911,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
         }
       }
       // ---- item epilogue
-      mbar_wait_bounded(pv_done, (g - 1) & 1u, abort_flag, status, DSV3_ERR_WAIT_TMEM);
+      pa_wait(pv_done, (g - 1) & 1u, abort_flag, status, DSV3_ERR_WAIT_TMEM);
       tc_fence_after();
       const bool whole = w.t0 == 0 && w.t1 == w.nt;
       const int slot = 2 * blockIdx.x + (w.t0 == 0 ? 1 : 0);
@@ -810,29 +920,31 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
         const int s0 = start->first + (count - w.left);
         my_rec = make_int4((int)row0, nr, (s0 + w.nt - 1) / start->share, 0);
       }
-      constexpr int W = NC < 32 ? NC : 32;
+      constexpr int WL = NC < L ? NC : L;            // columns of a group folded at a time
+      constexpr int GR = 32 / L;                     // groups of a half
 #pragma unroll
-      for (int c0 = 0; c0 < NC; c0 += W) {
-        const float v = fold_columns<W>(*reinterpret_cast<float(*)[W]>(&l[c0]), lane,
-                                        [](float x, float y) { return x + y; });
-        if (c0 > 0) half_sync(half);               // the last group is read
-        if (lane % (32 / W) == 0) myred[lane * W / 32 * 4 + (warp - 2 - 4 * half)] = v;
+      for (int c0 = 0; c0 < NC; c0 += WL) {
+        const float v = fold_columns<WL, L>(*reinterpret_cast<float(*)[WL]>(&l[c0]), lane,
+                                            [](float x, float y) { return x + y; });
+        if (c0 > 0) half_sync(half);               // the last columns are read
+        if (lane % (L / WL) == 0) myred[(group * WL + (lane & (L - 1)) * WL / L) * 4 + (warp - 2 - 4 * half)] = v;
         half_sync(half);
-        if (ht < W) {
+        if (ht < GR * WL) {
           const float4 r4 = *reinterpret_cast<const float4*>(myred + ht * 4);
           const float sum = (r4.x + r4.y) + (r4.z + r4.w);
-          const int n = col0 + c0 + ht;
+          const int n = half * NH + ht / WL * NC + c0 + ht % WL;
           if (!whole) part_ml[(size_t)slot * N + n] = make_float2(mref[n], sum);
           corr[n] = !whole ? 1.f : (sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum));
         }
       }
       half_sync(half);
+      constexpr int W = NH < 32 ? NH : 32;
       // O^T out: a thread holds one latent column of W rows; finished rows are
       // exchanged between neighbouring lanes and stored as bf16 pairs
 #pragma unroll 1
-      for (int i = 0; i < pl.LP * (NC / W); ++i) {
-        const int m = i / (NC / W), n0 = col0 + i % (NC / W) * W;
-        const int r = 128 * m + key;
+      for (int i = 0; i < pl.LP * (NH / W); ++i) {
+        const int m = i / (NH / W), n0 = half * NH + i % (NH / W) * W;
+        const int r = 128 * m + quarter * 32 + lane;
         if (n0 >= nr) continue;
         uint32_t o[W];
         tmem_ld_cols<W>(tmem + lane_base + (2 + m) * N + n0, o);
@@ -964,20 +1076,4 @@ __global__ void __launch_bounds__(FEW ? 512 : 256) paged_merge_kernel(const floa
     v.y = pack_bf16x2(acc.z * inv, acc.w * inv);
     *reinterpret_cast<uint2*>(out + (size_t)(rc.x + n) * R + r) = v;
   }
-}
-
-// Launch that may begin while its predecessor in the stream still runs; the
-// kernel waits for it (griddepcontrol.wait) before it reads anything.
-template <typename Kern, typename... Args>
-inline cudaError_t launch_dependent(Kern kern, dim3 grid, int block, cudaStream_t st, Args... args) {
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(block);
-  cfg.stream = st;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, args...);
 }
