@@ -1,6 +1,7 @@
 // Beam search: the choice of the next beams and the reordering of their cache.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <tuple>
@@ -16,7 +17,6 @@ namespace {
 typedef __nv_bfloat16 bf16;
 
 constexpr int kMaxBeams = 32;
-constexpr int kScanThreads = 256;
 constexpr int kPickThreads = 512;
 constexpr int kListCap = 512;      // candidates at or above a CTA's threshold that it ranks in shared memory
 
@@ -34,51 +34,69 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 __device__ __forceinline__ uint64_t entry_of(uint32_t key, uint32_t index) { return (uint64_t)key << 32 | ~index; }
 __device__ __forceinline__ uint32_t entry_index(uint64_t e) { return ~(uint32_t)e; }
 
-// A logit as the selection sees it: NaN counts as -inf, +inf as the largest
+// A logit as the selection sees it: NaN counts as -inf, +inf (below) as the largest
 // finite float, so that the log-sum-exp of a row is always defined.
-__device__ __forceinline__ float clean_logit(float x) { return fminf(fmaxf(x, -INFINITY), 3.402823466e38f); }
-__device__ __forceinline__ float clean_logit(bf16 x) { return clean_logit(__bfloat162float(x)); }
+constexpr float kLargest = 3.402823466e38f;
+__device__ __forceinline__ float number_of(float x) { return fmaxf(x, -INFINITY); }
+__device__ __forceinline__ float number_of(bf16 x) { return number_of(__bfloat162float(x)); }
 
-// The k best of a CTA's candidates.  The r-th largest of the lane maxima of each
-// warp, r = ceil(k / warps), is below at least k candidates, and so is the
-// smallest of these over the warps, the threshold: few candidates reach it
-// (22 of 8,192 for k = 8 on random data), and these are ranked by counting.
-// `top` is the lane's largest key, `each(f)` calls f(entry) for every candidate
-// of the thread.  Where more reach it than the list holds (many equal values) the
-// best are taken one at a time.  put(rank, entry) is called once per rank; a rank
-// without a candidate gets 0.
-template <int THREADS, typename Each, typename Put>
-__device__ __forceinline__ void cta_best(int k, uint32_t top, Each each, Put put) {
+// e^x for x <= 0, flushed to zero where it would be denormal.
+__device__ __forceinline__ float exp_of(float x) { return ex2_approx(x * 1.4426950408889634f); }
+
+// A key that at least k of a CTA's candidates reach and few more do (22 of 8,192
+// for k = 8 on random data): the k-th largest of the warps' maxima, or with fewer
+// than k warps the smallest over the warps of their r-th largest lane maximum, r =
+// ceil(k / warps).  `top` is the lane's largest key, 0 where it has none.  One
+// barrier.
+template <int THREADS>
+__device__ __forceinline__ uint32_t cta_threshold(int k, uint32_t top) {
   constexpr int W = THREADS / 32;
   __shared__ uint32_t s_low[W];
-  __shared__ uint64_t s_list[kListCap];
-  __shared__ int s_n;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int lane = threadIdx.x & 31;
   uint32_t left = top, low = 0;
   for (int i = 0; i < (k + W - 1) / W; ++i) {
     low = __reduce_max_sync(0xffffffffu, left);
     const unsigned who = __ballot_sync(0xffffffffu, left == low);
     if (lane == __ffs(who) - 1) left = 0;
   }
-  if (lane == 0) s_low[warp] = low;
-  if (tid == 0) s_n = 0;
+  if (lane == 0) s_low[threadIdx.x >> 5] = low;
   __syncthreads();
-  uint32_t threshold = s_low[0];
+  const int me = lane & (W - 1);
+  const uint32_t mine = s_low[me];
+  if (k > W) return __reduce_min_sync(0xffffffffu, mine);
+  int rank = 0;
 #pragma unroll
-  for (int w = 1; w < W; ++w) threshold = min(threshold, s_low[w]);
-  if (top >= threshold && top > 0)
-    each([&](uint64_t e) {
-      if ((uint32_t)(e >> 32) >= threshold && e >> 32) {
-        const int at = atomicAdd(&s_n, 1);
-        if (at < kListCap) s_list[at] = e;
-      }
+  for (int w = 0; w < W; ++w) {
+    const uint32_t other = __shfl_sync(0xffffffffu, mine, w);
+    rank += other > mine || (other == mine && w < me);
+  }
+  return __shfl_sync(0xffffffffu, mine, __ffs(__ballot_sync(0xffffffffu, rank == k - 1)) - 1);
+}
+
+// The k best of the candidates whose key reaches `threshold`, ranked by counting
+// in shared memory.  `each(least, f)` calls f(entry) for the thread's candidates
+// whose key is `least` or more; `any` says whether it may have one.
+// Where more reach the threshold than the list holds (many equal values) the best
+// are taken one at a time.  put(rank, entry) is called once per rank; a rank
+// without a candidate gets 0.  *s_n is 0 on entry, and the caller's barrier comes
+// before the next use.
+template <int THREADS, typename Each, typename Put>
+__device__ __forceinline__ void cta_rank(int k, uint32_t threshold, bool any, int* s_n, Each each, Put put) {
+  constexpr int W = THREADS / 32;
+  __shared__ uint64_t s_list[kListCap];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (any)
+    each(max(threshold, 1u), [&](uint64_t e) {
+      const int at = atomicAdd(s_n, 1);
+      if (at < kListCap) s_list[at] = e;
     });
   __syncthreads();
-  const int n = s_n;
+  const int n = *s_n;
   if (n <= kListCap) {
     for (int i = tid; i < n; i += THREADS) {
       const uint64_t e = s_list[i];
       int rank = 0;
+#pragma unroll 4
       for (int j = 0; j < n; ++j) rank += s_list[j] > e;
       if (rank < k) put(rank, e);
     }
@@ -88,7 +106,7 @@ __device__ __forceinline__ void cta_best(int k, uint32_t top, Each each, Put put
   uint64_t last = ~(uint64_t)0;
   for (int r = 0; r < k; ++r) {
     uint64_t best = 0;
-    each([&](uint64_t e) {
+    each(1u, [&](uint64_t e) {
       if (e < last && e > best) best = e;
     });
 #pragma unroll
@@ -106,82 +124,139 @@ __device__ __forceinline__ void cta_best(int k, uint32_t top, Each each, Put put
   }
 }
 
-// 16 bytes at an address that is `align` (0, 4, 8 or 12) modulo 16.
-__device__ __forceinline__ uint4 load_16_bytes(const void* p, int align) {
-  if (align == 0) return __ldg(reinterpret_cast<const uint4*>(p));
-  uint4 u;
-  if (align == 8) {
-    const uint2 a = __ldg(reinterpret_cast<const uint2*>(p)), b = __ldg(reinterpret_cast<const uint2*>(p) + 1);
-    u = make_uint4(a.x, a.y, b.x, b.y);
-  } else {
-    const uint32_t* q = reinterpret_cast<const uint32_t*>(p);
-    u = make_uint4(__ldg(q), __ldg(q + 1), __ldg(q + 2), __ldg(q + 3));
-  }
-  return u;
-}
-
-// One CTA per (segment, row): maximum, sum of exponentials and the k largest of
-// PER * 256 logits, which stay in registers between one read and the rest.  A
-// thread's elements go by their index in the row, never by its address, so that
-// sums and scores are the same wherever a row lies.  Bound by reading the
-// logits (32 x 8 rows of 102,400 fp32: 16 us at the copy rate).
-template <typename T, int PER>
-__global__ void __launch_bounds__(kScanThreads) beam_scan_kernel(const T* __restrict__ logits, long ldb, long ldk, int K,
-                                                                 int V, const bool* __restrict__ finished,
-                                                                 float2* __restrict__ stat,
-                                                                 uint64_t* __restrict__ cand) {
-  constexpr int VE = 16 / sizeof(T), NV = PER / VE;
+// A CTA walks `chunk` consecutive segments of PER * THREADS logits, rows one after
+// another, and leaves one record per row that it touches: maximum, sum of
+// exponentials and the K largest of its part.  Every thread keeps a running
+// maximum and sum, the CTA a list of the K best so far; a segment that holds
+// nothing above the last of them costs one barrier.  The logits of the next
+// segment are on their way while this one is looked at.  A thread's elements go
+// by their index in the row, never by its address, so that sums and scores are
+// the same wherever a row lies.  Bound by reading the logits.
+template <typename T, int THREADS, int PER, bool ALIGNED>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) beam_scan_kernel(const T* __restrict__ logits, long ldb, long ldk,
+                                                                            int units, int nseg, int chunk, int runs,
+                                                                            int K, int V,
+                                                                            const bool* __restrict__ finished,
+                                                                            float2* __restrict__ stat,
+                                                                            uint64_t* __restrict__ cand) {
+  constexpr int VE = 16 / sizeof(T), NV = PER / VE, W = THREADS / 32;
+  __shared__ float2 red[W];
+  __shared__ uint64_t best[2][kMaxBeams];
+  __shared__ int s_n;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int row = blockIdx.y, seg = blockIdx.x, nseg = gridDim.x;
-  if (finished != nullptr && finished[row]) return;
-  const T* x = logits + (row / K) * ldb + (row % K) * ldk;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int align = (int)(reinterpret_cast<uintptr_t>(x) & 15);
-  const int first = seg * PER * kScanThreads + tid * VE;
-  float v[PER];
+  const int u0 = blockIdx.x * chunk, u1 = min(u0 + chunk, units);
+  uint4 raw[NV];                          // of the next segment, as loaded
+  int row = u0 / nseg, seg = u0 % nseg;   // that segment
+  const bool even = ldb == ldk * K;       // rows at one stride
+  // Loads it: by 16 bytes, by 4 bytes where rows are not all ALIGNED, and what a
+  // row does not fill, or a row at an odd address, element by element.  False where
+  // the row is finished.
+  auto fetch = [&]() {
+    if (finished != nullptr && finished[row]) return false;
+    const T* x = logits + (even ? row * ldk : (row / K) * ldb + (row % K) * ldk);
+    const int first = seg * PER * THREADS + tid * VE;
+    if ((seg + 1) * PER * THREADS <= V && (ALIGNED || (reinterpret_cast<uintptr_t>(x) & 3) == 0)) {
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int at = first + j * kScanThreads * VE;
-    if (at + VE <= V && align % 4 == 0) {
-      const uint4 u = load_16_bytes(x + at, align);
-      const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-      for (int i = 0; i < VE; ++i) v[j * VE + i] = clean_logit(e[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < VE; ++i) v[j * VE + i] = at + i < V ? clean_logit(x[at + i]) : -INFINITY;
-    }
-  }
-  __shared__ float red[2][kScanThreads / 32];
-  float tmax = v[0];
-#pragma unroll
-  for (int i = 1; i < PER; ++i) tmax = fmaxf(tmax, v[i]);
-  float mx = warp_max(tmax);
-  if (lane == 0) red[0][warp] = mx;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kScanThreads / 32; ++i) mx = fmaxf(mx, red[0][i]);
-  mx = fmaxf(mx, -3.402823466e38f);
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) s += __expf(v[i] - mx);
-  s = warp_sum(s);
-  if (lane == 0) red[1][warp] = s;
-  uint64_t* o = cand + ((size_t)row * nseg + seg) * K;
-  cta_best<kScanThreads>(
-      K, first < V ? order_key(tmax) : 0u,
-      [&](auto&& f) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const int at = first + (i / VE) * kScanThreads * VE + i % VE;
-          if (at < V) f(entry_of(order_key(v[i]), (uint32_t)at));
+      for (int j = 0; j < NV; ++j) {
+        const T* p = x + first + j * THREADS * VE;
+        if constexpr (ALIGNED) {
+          raw[j] = __ldg(reinterpret_cast<const uint4*>(p));
+        } else {
+          const uint32_t* q = reinterpret_cast<const uint32_t*>(p);
+          raw[j] = make_uint4(__ldg(q), __ldg(q + 1), __ldg(q + 2), __ldg(q + 3));
         }
-      },
-      [&](int rank, uint64_t e) { o[rank] = e; });
-  if (tid == 0) {                         // the barriers of cta_best lie between
-    float t = 0.f;
-    for (int i = 0; i < kScanThreads / 32; ++i) t += red[1][i];
-    stat[(size_t)row * nseg + seg] = make_float2(mx, t);
+      }
+    } else {
+      const T low = (T)-INFINITY;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        T* e = reinterpret_cast<T*>(&raw[j]);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+          const int at = first + j * THREADS * VE + i;
+          e[i] = at < V ? x[at] : low;
+        }
+      }
+    }
+    return true;
+  };
+  bool next_live = u0 < u1 && fetch();
+  float m = -kLargest, s = 0.f;
+  uint32_t last = 0;                      // key of the K-th best so far
+  int cur = 0;
+  for (int u = u0; u < u1; ++u) {
+    const bool live = next_live, begin = u == u0 || seg == 0, end = u + 1 == u1 || seg == nseg - 1;
+    const int first = seg * PER * THREADS + tid * VE, this_row = row;
+    float v[PER];
+    if (live) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < VE; ++i) v[j * VE + i] = number_of(reinterpret_cast<const T*>(&raw[j])[i]);
+    }
+    if (u + 1 < u1) {
+      if (++seg == nseg) {
+        seg = 0;
+        ++row;
+      }
+      next_live = fetch();
+    }
+    if (!live) continue;
+    float top = v[0];
+#pragma unroll
+    for (int i = 1; i < PER; ++i) top = fmaxf(top, v[i]);
+    if (top > kLargest) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) v[i] = fminf(v[i], kLargest);
+      top = kLargest;
+    }
+    if (begin) {
+      m = -kLargest;
+      s = 0.f;
+    }
+    const float now = fmaxf(m, top);
+    s *= exp_of(m - now);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) s += exp_of(v[i] - now);
+    m = now;
+    const uint32_t key = first < V ? order_key(top) : 0u;
+    if (tid == 0) s_n = 0;
+    const uint32_t threshold = begin ? cta_threshold<THREADS>(K, key) : last + 1;   // later indices lose ties
+    const bool any = key >= threshold && key > 0;
+    if (begin || __syncthreads_or(any)) {
+      cta_rank<THREADS>(
+          K, threshold, any || (!begin && tid < K), &s_n,
+          [&](uint32_t least, auto&& f) {
+            const float low = key_value(least);          // (a NaN for keys below that of -inf)
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+              if (!(v[i] < low)) {
+                const int at = first + (i / VE) * THREADS * VE + i % VE;
+                const uint32_t k = order_key(v[i]);
+                if (at < V && k >= least) f(entry_of(k, (uint32_t)at));
+              }
+            if (!begin && tid < K && best[cur][tid] != 0) f(best[cur][tid]);
+          },
+          [&](int rank, uint64_t e) { best[cur ^ 1][rank] = e; });
+      __syncthreads();
+      cur ^= 1;
+      last = (uint32_t)(best[cur][K - 1] >> 32);
+    }
+    if (end) {
+      const float wm = warp_max(m);
+      const float ws = warp_sum(s * exp_of(m - wm));
+      if (lane == 0) red[warp] = make_float2(wm, ws);
+      __syncthreads();
+      const size_t at = (size_t)this_row * runs + (blockIdx.x - this_row * nseg / chunk);
+      if (tid < K) cand[at * K + tid] = best[cur][tid];
+      if (warp == W - 1) {
+        const float2 r = lane < W ? red[lane] : make_float2(-kLargest, 0.f);
+        const float M = warp_max(r.x);
+        const float sum = warp_sum(r.y * exp_of(r.x - M));
+        if (lane == 0) stat[at] = make_float2(M, sum);
+      }
+    }
   }
 }
 
@@ -190,22 +265,25 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const float2* _
                                                                  const uint64_t* __restrict__ cand,
                                                                  const float* __restrict__ scores,
                                                                  const bool* __restrict__ finished, int K, int V,
-                                                                 int nseg, int eos, float* __restrict__ o_score,
+                                                                 int nseg, int chunk, int runs, int eos,
+                                                                 float* __restrict__ o_score,
                                                                  int* __restrict__ o_parent, int* __restrict__ o_token,
                                                                  bool* __restrict__ o_done) {
   const int b = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   __shared__ float s_max[kMaxBeams], s_log[kMaxBeams], s_score[kMaxBeams];
   __shared__ bool s_done[kMaxBeams];
+  __shared__ int s_runs[kMaxBeams], s_n;
   const size_t row0 = (size_t)b * K;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   for (int r = warp; r < K; r += kPickThreads / 32) {
     const bool done = finished != nullptr && finished[row0 + r];
-    const float2* st = stat + (row0 + r) * nseg;
-    float m = -3.402823466e38f, s = 0.f;
+    const float2* st = stat + (row0 + r) * runs;
+    const int row = (int)row0 + r, n = ((row + 1) * nseg - 1) / chunk - row * nseg / chunk + 1;   // parts of the row
+    float m = -kLargest, s = 0.f;
     if (!done) {
-      for (int i = lane; i < nseg; i += 32) m = fmaxf(m, st[i].x);
+      for (int i = lane; i < n; i += 32) m = fmaxf(m, st[i].x);
       m = warp_max(m);
-      for (int i = lane; i < nseg; i += 32) s += st[i].y * expf(st[i].x - m);
+      for (int i = lane; i < n; i += 32) s += st[i].y * expf(st[i].x - m);
       s = warp_sum(s);
     }
     if (lane == 0) {
@@ -213,10 +291,12 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const float2* _
       s_log[r] = logf(s);
       s_score[r] = scores[row0 + r];
       s_done[r] = done;
+      s_runs[r] = n;
     }
   }
+  if (tid == 0) s_n = 0;
   __syncthreads();
-  const int per = nseg * K;               // candidates per beam
+  const int per = runs * K;               // candidates per beam, at most
   auto candidate = [&](int c) -> uint64_t {
     const int r = c / per, i = c % per;
     const float sc = s_score[r];
@@ -230,6 +310,7 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const float2* _
       if (i >= K) return 0;
       v = i;
     } else {
+      if (i >= s_runs[r] * K) return 0;
       const uint64_t e = cand[row0 * per + c];
       if (e == 0) return 0;
       v = entry_index(e);
@@ -239,10 +320,14 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const float2* _
   };
   uint32_t top = 0;
   for (int c = tid; c < K * per; c += kPickThreads) top = max(top, (uint32_t)(candidate(c) >> 32));
-  cta_best<kPickThreads>(
-      K, top,
-      [&](auto&& f) {
-        for (int c = tid; c < K * per; c += kPickThreads) f(candidate(c));
+  const uint32_t threshold = cta_threshold<kPickThreads>(K, top);
+  cta_rank<kPickThreads>(
+      K, threshold, top >= threshold && top > 0, &s_n,
+      [&](uint32_t least, auto&& f) {
+        for (int c = tid; c < K * per; c += kPickThreads) {
+          const uint64_t e = candidate(c);
+          if (e >> 32 >= least) f(e);
+        }
       },
       [&](int rank, uint64_t e) {
         const uint32_t at = entry_index(e);
@@ -358,39 +443,48 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> beam_select(const at:
     TORCH_CHECK(eos >= 0 && eos < V, op, ": finished beams need an end token inside the vocabulary");
     done = finished->data_ptr<bool>();
   }
-  TORCH_CHECK(B * K <= 65535, op, ": too many rows");
+  TORCH_CHECK(B * K * ((V + 2047) / 2048) < (1ll << 31), op, ": too many rows");
   const at::cuda::CUDAGuard guard(logits.device());
   auto st = at::cuda::getCurrentCUDAStream();
-  auto iopt = scores.options().dtype(at::kInt);
-  auto o_score = at::empty({B, K}, scores.options()), o_parent = at::empty({B, K}, iopt),
-       o_token = at::empty({B, K}, iopt), o_done = at::empty({B, K}, scores.options().dtype(at::kBool));
+  // (straight to the allocator: five tensors through the dispatcher cost more
+  // host time than the two launches)
+  auto make = [&](at::IntArrayRef sizes, at::ScalarType t) {
+    return at::Tensor(at::detail::empty_cuda(sizes, t, logits.device(), c10::nullopt));
+  };
+  auto o_score = make({B, K}, at::kFloat), o_parent = make({B, K}, at::kInt), o_token = make({B, K}, at::kInt),
+       o_done = make({B, K}, at::kBool);
   if (B == 0) return {o_score, o_parent, o_token, o_done};
-  // 32 logits per thread where that gives two CTAs per SM, else 8: with few rows
-  // the latency of a segment counts, not its overhead (4 rows of 100,018: 12 us
-  // against 15 us)
-  const int64_t sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  const int per = B * K * ((V + 32 * kScanThreads - 1) / (32 * kScanThreads)) >= 2 * sms ? 32 : 8;
-  const int nseg = (int)((V + per * kScanThreads - 1) / (per * kScanThreads));
-  auto work = at::empty({B * K * nseg * (1 + K) * 2}, scores.options());
+  // segments of 4,096 logits where that gives four CTAs per SM, else of 2,048: with
+  // few rows the latency of a segment counts, not its overhead
+  const int64_t sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount, es = logits.element_size();
+  const int span = B * K * ((V + 4095) / 4096) >= 4 * sms ? 4096 : 2048;
+  const int nseg = (int)((V + span - 1) / span);
+  const bool aligned = reinterpret_cast<uintptr_t>(logits.data_ptr()) % 16 == 0 && logits.stride(0) * es % 16 == 0 &&
+                       logits.stride(1) * es % 16 == 0;
+  const int64_t units = B * K * nseg, ctas = sms * 4;
+  const int chunk = (int)((units + ctas - 1) / ctas), runs = (nseg - 1) / chunk + 2;   // parts of a row, at most
+  auto work = make({B * K * runs * (1 + K) * 2}, at::kFloat);
   float2* stat = reinterpret_cast<float2*>(work.data_ptr());
-  uint64_t* cand = reinterpret_cast<uint64_t*>(stat + B * K * nseg);
-  const dim3 grid(nseg, (unsigned)(B * K));
-#define DSV3_SCAN(T_, PER_)                                                                                   \
-  beam_scan_kernel<T_, PER_><<<grid, kScanThreads, 0, st>>>(reinterpret_cast<const T_*>(logits.data_ptr()),  \
-                                                            logits.stride(0), logits.stride(1), (int)K,      \
-                                                            (int)V, done, stat, cand)
-  if (logits.scalar_type() == at::kFloat) {
-    if (per == 32) DSV3_SCAN(float, 32);
-    else DSV3_SCAN(float, 8);
-  } else {
-    if (per == 32) DSV3_SCAN(bf16, 32);
-    else DSV3_SCAN(bf16, 8);
-  }
+  uint64_t* cand = reinterpret_cast<uint64_t*>(stat + B * K * runs);
+#define DSV3_SCAN(T_, PER_, ALIGNED_)                                                                          \
+  beam_scan_kernel<T_, 256, PER_, ALIGNED_><<<(unsigned)((units + chunk - 1) / chunk), 256, 0, st>>>(          \
+      reinterpret_cast<const T_*>(logits.data_ptr()), logits.stride(0), logits.stride(1), (int)units, nseg, chunk, \
+      runs, (int)K, (int)V, done, stat, cand)
+#define DSV3_SCAN_TYPE(T_)                              \
+  do {                                                  \
+    if (span == 4096 && aligned) DSV3_SCAN(T_, 16, true); \
+    else if (span == 4096) DSV3_SCAN(T_, 16, false);    \
+    else if (aligned) DSV3_SCAN(T_, 8, true);           \
+    else DSV3_SCAN(T_, 8, false);                       \
+  } while (0)
+  if (logits.scalar_type() == at::kFloat) DSV3_SCAN_TYPE(float);
+  else DSV3_SCAN_TYPE(bf16);
+#undef DSV3_SCAN_TYPE
 #undef DSV3_SCAN
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   C10_CUDA_CHECK(launch_dependent(beam_pick_kernel, dim3((unsigned)B), kPickThreads, st, (const float2*)stat,
                                   (const uint64_t*)cand, (const float*)scores.data_ptr<float>(), done, (int)K, (int)V,
-                                  nseg, (int)eos, o_score.data_ptr<float>(), o_parent.data_ptr<int>(),
+                                  nseg, chunk, runs, (int)eos, o_score.data_ptr<float>(), o_parent.data_ptr<int>(),
                                   o_token.data_ptr<int>(), o_done.data_ptr<bool>()));
   return {o_score, o_parent, o_token, o_done};
 }
@@ -417,7 +511,7 @@ at::Tensor beam_reorder(at::Tensor& pages, const at::Tensor& table, const at::Te
               op, ": seq_lens must be a contiguous int32 tensor [B]");
   TORCH_CHECK(B <= 65535 && pages.size(0) <= 65535 && pages.size(1) < (1ll << 31), op, ": too many groups or layers");
   const at::cuda::CUDAGuard guard(pages.device());
-  auto out = at::empty({B * K, table.size(1)}, table.options());
+  auto out = at::Tensor(at::detail::empty_cuda({B * K, table.size(1)}, at::kInt, pages.device(), c10::nullopt));
   if (B == 0 || table.size(1) == 0) return out;
   const int row16 = (int)(width * es / 16);
   const int parts = (int)((page * row16 + kCopyThreads * kCopyVecs - 1) / (kCopyThreads * kCopyVecs));

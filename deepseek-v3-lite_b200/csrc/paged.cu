@@ -18,8 +18,10 @@
 // batch's offsets is skipped and recorded in the device status word.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <atomic>
 #include <string>
 
 #include "common.cuh"
@@ -98,6 +100,18 @@ __global__ void __launch_bounds__(128) latent_append_kernel(const T* __restrict_
 #include "paged_attention_tc.cuh"
 
 // --------------------------------------------------------------- host side
+// Opt a kernel in to the full shared memory of a CTA, once per device (the call
+// costs host time on every launch otherwise).
+template <typename Kern>
+void allow_shared_memory(Kern kern, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  C10_CUDA_CHECK(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_acquire) & bit) return;
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPaSmem));
+  done.fetch_or(bit, std::memory_order_release);
+}
+
 Ragged check_ragged(const char* op, const at::Tensor& ref, const at::Tensor& pages, const at::Tensor& table,
                     const at::Tensor& cu, const at::Tensor& lens) {
   TORCH_CHECK(pages.is_cuda() && pages.dim() == 3 && pages.scalar_type() == at::kBFloat16 && pages.stride(2) == 1,
@@ -185,7 +199,7 @@ at::Tensor paged_latent_attention(const at::Tensor& q, const at::Tensor& pages, 
               std::to_string(R), " and ", std::to_string(D - R));
   TORCH_CHECK(H >= 1 && H <= 4096 && T * H < (1ll << 31), op, ": 1 to 4096 heads and T * H below 2^31");
   TORCH_CHECK(scale > 0, op, ": scale must be positive");
-  auto out = at::empty({T, H, R}, q.options());
+  auto out = at::Tensor(at::detail::empty_cuda({T, H, R}, at::kBFloat16, pages.device(), c10::nullopt));
   if (T == 0) return out;
   TORCH_CHECK(rg.B > 0, op, ": tokens without a sequence");
   const at::cuda::CUDAGuard guard(pages.device());
@@ -198,7 +212,8 @@ at::Tensor paged_latent_attention(const at::Tensor& q, const at::Tensor& pages, 
   constexpr int KT = 64;
   PagedPlan pl;
   TORCH_CHECK(paged_plan(N, KT, (int)R, (int)D, pl), op, ": no shared-memory plan");
-  auto work = at::empty({sms * (2 * N * (R + 2) + 4)}, q.options().dtype(at::kFloat));
+  auto work = at::Tensor(
+      at::detail::empty_cuda({sms * (2 * N * (R + 2) + 4)}, at::kFloat, pages.device(), c10::nullopt));
   int4* rec = reinterpret_cast<int4*>(work.data_ptr<float>());
   float2* ml = reinterpret_cast<float2*>(rec + sms);
   float* part = reinterpret_cast<float*>(ml + 2 * (int64_t)sms * N);
@@ -213,10 +228,11 @@ at::Tensor paged_latent_attention(const at::Tensor& q, const at::Tensor& pages, 
   const int64_t cuts = std::min<int64_t>(sms, T * H / N + rg.B);   // row tiles that can be cut, at most
   const bool few = cuts * 4 <= sms;
   bf16* o = reinterpret_cast<bf16*>(out.data_ptr());
+  static std::atomic<uint64_t> opted[4];   // devices on which each variant may take all shared memory
+  const int variant = N == 16 ? 0 : N == 32 ? 1 : N == 64 ? 2 : 3;
 #define DSV3_PAGED(N_, KT_)                                                                                           \
   do {                                                                                                           \
-    C10_CUDA_CHECK(cudaFuncSetAttribute(paged_attention_tc_kernel<N_, KT_>,                                           \
-                                        cudaFuncAttributeMaxDynamicSharedMemorySize, pl.smem));                  \
+    allow_shared_memory(paged_attention_tc_kernel<N_, KT_>, opted[variant]);                                      \
     paged_attention_tc_kernel<N_, KT_><<<sms, kPaThreads, pl.smem, st>>>(                                             \
         tm_q, tm_kv, pl, rg, (int)T, (int)H, (int)R, (int)D, (float)(scale * 1.4426950408889634), 1, o, part, ml, \
         rec, status_ptr());                                                                                      \

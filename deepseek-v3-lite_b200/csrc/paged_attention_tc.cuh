@@ -42,6 +42,7 @@
 
 constexpr int kPaThreads = 352;
 constexpr int kPaMaxSlots = 16;
+constexpr int kPaSmem = 232448;              // shared memory of a CTA, at most
 constexpr float kPaUnset = -1e30f;           // reference of a row that has seen no key
 constexpr float kPaLead = 12.f;              // first reference above the first key's score (log2)
 
@@ -61,7 +62,7 @@ inline bool paged_plan(int N, int KT, int R, int D, PagedPlan& p) {
   p.tail = D > 128 * p.LP ? 1 : 0;
   p.tails = p.tail ? 2 : 0;
   const int q = p.nch * N * 128, P = (N + 63) / 64 * chunk, misc = 12 * N + 1024 + 512;
-  const int fit = (232448 - q - P - p.tails * chunk - misc) / (2 * chunk);
+  const int fit = (kPaSmem - q - P - p.tails * chunk - misc) / (2 * chunk);
   p.slots = fit < kPaMaxSlots ? fit : kPaMaxSlots;
   p.off_t = p.slots * 2 * chunk;
   p.off_p = p.off_t + p.tails * chunk;

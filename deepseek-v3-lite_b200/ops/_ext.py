@@ -40,6 +40,7 @@ class _CountingModule:
                     _counting[1] += n
                 return fn(*a, **k)
             self._cache[name] = w
+            self.__dict__[name] = w     # later look-ups skip this method
         return w
 
 
