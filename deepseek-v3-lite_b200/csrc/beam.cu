@@ -133,7 +133,7 @@ __device__ __forceinline__ void cta_rank(int k, uint32_t threshold, bool any, in
 // by their index in the row, never by its address, so that sums and scores are
 // the same wherever a row lies.  Bound by reading the logits.
 template <typename T, int THREADS, int PER, bool ALIGNED>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) beam_scan_kernel(const T* __restrict__ logits, long ldb, long ldk,
+__global__ void __launch_bounds__(THREADS, 3) beam_scan_kernel(const T* __restrict__ logits, long ldb, long ldk,
                                                                             int units, int nseg, int chunk, int runs,
                                                                             int K, int V,
                                                                             const bool* __restrict__ finished,
@@ -454,14 +454,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> beam_select(const at:
   auto o_score = make({B, K}, at::kFloat), o_parent = make({B, K}, at::kInt), o_token = make({B, K}, at::kInt),
        o_done = make({B, K}, at::kBool);
   if (B == 0) return {o_score, o_parent, o_token, o_done};
-  // segments of 4,096 logits where that gives four CTAs per SM, else of 2,048: with
+  // segments of 4,096 logits where that gives three CTAs per SM, else of 2,048: with
   // few rows the latency of a segment counts, not its overhead
   const int64_t sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount, es = logits.element_size();
-  const int span = B * K * ((V + 4095) / 4096) >= 4 * sms ? 4096 : 2048;
+  const int span = B * K * ((V + 4095) / 4096) >= 3 * sms ? 4096 : 2048;
   const int nseg = (int)((V + span - 1) / span);
   const bool aligned = reinterpret_cast<uintptr_t>(logits.data_ptr()) % 16 == 0 && logits.stride(0) * es % 16 == 0 &&
                        logits.stride(1) * es % 16 == 0;
-  const int64_t units = B * K * nseg, ctas = sms * 4;
+  const int64_t units = B * K * nseg, ctas = sms * 3;
   const int chunk = (int)((units + ctas - 1) / ctas), runs = (nseg - 1) / chunk + 2;   // parts of a row, at most
   auto work = make({B * K * runs * (1 + K) * 2}, at::kFloat);
   float2* stat = reinterpret_cast<float2*>(work.data_ptr());
