@@ -233,7 +233,7 @@ at::Tensor paged_latent_attention(const at::Tensor& q, const at::Tensor& pages, 
 #define DSV3_PAGED(N_, KT_)                                                                                           \
   do {                                                                                                           \
     allow_shared_memory(paged_attention_tc_kernel<N_, KT_>, opted[variant]);                                      \
-    paged_attention_tc_kernel<N_, KT_><<<sms, kPaThreads, pl.smem, st>>>(                                             \
+    paged_attention_tc_kernel<N_, KT_><<<sms, pa_threads(N_), pl.smem, st>>>(                                             \
         tm_q, tm_kv, pl, rg, (int)T, (int)H, (int)R, (int)D, (float)(scale * 1.4426950408889634), 1, o, part, ml, \
         rec, status_ptr());                                                                                      \
     C10_CUDA_KERNEL_LAUNCH_CHECK();                                                                              \

@@ -35,12 +35,16 @@
 // which a second kernel merges in share order, so results do not depend on
 // timing.
 //
-// Warps: 0 TMA, 1 first product (and TMEM), 2..9 softmax and epilogue, 10 second
-// product.  Every wait is
+// Warps: 0 TMA, 1 first product (and TMEM), then two or four warpgroups of softmax
+// and epilogue, and one warp for the second product.  Every wait is
 // bounded; after one ran out the softmax warps go on without waiting, so that
 // they meet at their barriers, and the others stop.
 
-constexpr int kPaThreads = 352;
+// Softmax warpgroups of a row tile, each with its share of the rows: two for few
+// rows; four for 64 and 128, where two spent longer on a tile than the tensor core
+// (2,200 cycles against 1,400 for 128 rows).
+constexpr int pa_groups(int N) { return N >= 64 ? 4 : 2; }
+constexpr int pa_threads(int N) { return 32 * (3 + 4 * pa_groups(N)); }   // TMA, S, softmax, PV
 constexpr int kPaMaxSlots = 16;
 constexpr int kPaSmem = 232448;              // shared memory of a CTA, at most
 constexpr float kPaUnset = -1e30f;           // reference of a row that has seen no key
@@ -49,6 +53,7 @@ constexpr float kPaLead = 12.f;              // first reference above the first 
 struct PagedPlan {
   int LP, nch, tail;          // latent chunk pairs, chunks, 1 if there is a tail chunk
   int slots, tails;           // ring slots (pairs), tail slots
+  int pbufs;                  // buffers of P
   int off_q, off_p, off_t, off_misc, smem, tmem_cols;
 };
 
@@ -61,12 +66,16 @@ inline bool paged_plan(int N, int KT, int R, int D, PagedPlan& p) {
   p.nch = (D + 63) / 64;
   p.tail = D > 128 * p.LP ? 1 : 0;
   p.tails = p.tail ? 2 : 0;
-  const int q = p.nch * N * 128, P = (N + 63) / 64 * chunk, misc = 12 * N + 1024 + 512;
-  const int fit = (kPaSmem - q - P - p.tails * chunk - misc) / (2 * chunk);
-  p.slots = fit < kPaMaxSlots ? fit : kPaMaxSlots;
+  const int q = p.nch * N * 128, P = (N + 63) / 64 * chunk, misc = 28 * N + 520;
+  // a second P buffer where the ring still holds two key tiles with it
+  for (p.pbufs = 2;; --p.pbufs) {
+    const int fit = (kPaSmem - q - p.pbufs * P - p.tails * chunk - misc) / (2 * chunk);
+    p.slots = fit < kPaMaxSlots ? fit : kPaMaxSlots;
+    if (p.slots >= 2 * p.LP || p.pbufs == 1) break;
+  }
   p.off_t = p.slots * 2 * chunk;
   p.off_p = p.off_t + p.tails * chunk;
-  p.off_q = p.off_p + P;
+  p.off_q = p.off_p + p.pbufs * P;
   p.off_misc = p.off_q + q;
   p.smem = p.off_misc + misc;
   p.tmem_cols = 32;
@@ -286,17 +295,17 @@ struct PagedStart {
 template <int N, int KT>
 __device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, int min_share, PagedStart* out, int* scan, unsigned int* status) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr int NW = kPaThreads / 32;
+  constexpr int THREADS = pa_threads(N), NW = THREADS / 32;
   // round 0 adds up all sequences; round 1 finds the one that holds the share's
-  // first tile (a batch of up to kPaThreads sequences is still in registers)
+  // first tile (a batch of up to THREADS sequences is still in registers)
   int target = 0, t = 0;
   PagedSeq s;
   s.tiles = 0;
   for (int round = 0; round < 2; ++round) {
     int base = 0;
-    for (int b0 = 0; b0 < r.B; b0 += kPaThreads) {
+    for (int b0 = 0; b0 < r.B; b0 += THREADS) {
       const int b = b0 + tid;
-      if (round == 0 || r.B > kPaThreads) {
+      if (round == 0 || r.B > THREADS) {
         s.tiles = 0;
         t = 0;
         if (b < r.B) {
@@ -357,7 +366,7 @@ __device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, in
     s = paged_seq<N>(r, out->b, H, total);
     int lo = 0, hi = s.tiles;                    // the answer lies in [lo, hi)
     while (hi > lo) {
-      const int step = (hi - lo + kPaThreads - 1) / kPaThreads, k = lo + tid * step;
+      const int step = (hi - lo + THREADS - 1) / THREADS, k = lo + tid * step;
       const int k1 = min(k + step, hi);
       if (k < hi) {
         const long long at = paged_tiles_before<N, KT>(s, k, H);
@@ -507,18 +516,19 @@ struct Ring {
 };
 
 template <int N, int KT>
-__global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
+__global__ void __launch_bounds__(pa_threads(N), 1) paged_attention_tc_kernel(
     const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ PagedPlan pl,
     const __grid_constant__ Ragged rg,
     int total, int H, int R, int D, float scale_log2, int min_share, bf16* __restrict__ out,
     float* __restrict__ part_o, float2* __restrict__ part_ml, int4* __restrict__ rec, unsigned int* status) {
+  constexpr int G = pa_groups(N), PBUF = (N + 63) / 64 * KT * 128;
   constexpr int CHUNK = KT * 128, PAIR = 2 * CHUNK;  // [KT keys x 64 columns], two of them (bytes)
   extern __shared__ __align__(1024) uint8_t smem[];
   float* mref = reinterpret_cast<float*>(smem + pl.off_misc);            // [N]
   int* lim = reinterpret_cast<int*>(mref + N);                           // [N] keys that a row sees
   float* corr = reinterpret_cast<float*>(lim + N);                       // [N] rescaling, 1 / sum, or maximum keys
-  float* red = corr + N;                                                 // [2][32][4]
-  uint64_t* pair_full = reinterpret_cast<uint64_t*>(red + 256);
+  float* red = corr + N;                                                 // [N][4]
+  uint64_t* pair_full = reinterpret_cast<uint64_t*>(red + 4 * N);
   uint64_t* pair_empty = pair_full + kPaMaxSlots;
   uint64_t* tail_full = pair_empty + kPaMaxSlots;
   uint64_t* tail_empty = tail_full + 2;
@@ -526,13 +536,13 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
   uint64_t* q_empty = q_full + 1;
   uint64_t* s_full = q_empty + 1;     // [2]
   uint64_t* p_ready = s_full + 2;
-  uint64_t* pv_done = p_ready + 1;
-  uint64_t* o_free = pv_done + 1;
+  uint64_t* pv_done = p_ready + 2;    // p_ready, pv_done, s_full, s_free: one per parity of the tile
+  uint64_t* o_free = pv_done + 2;
   uint64_t* s_free = o_free + 1;      // [2]
   uint64_t* drain = s_free + 2;       // [2]
   PagedStart* start = reinterpret_cast<PagedStart*>(drain + 2);
-  int* scan = reinterpret_cast<int*>(start + 1);             // [kPaThreads / 32]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(scan + kPaThreads / 32);
+  int* scan = reinterpret_cast<int*>(start + 1);             // [threads / 32]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(scan + pa_threads(N) / 32);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -549,11 +559,13 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
     mbar_init(q_empty, 1);
     mbar_init(&s_full[0], 1);
     mbar_init(&s_full[1], 1);
-    mbar_init(p_ready, 8);
-    mbar_init(pv_done, 1);
-    mbar_init(o_free, 8);
-    mbar_init(&s_free[0], 8);
-    mbar_init(&s_free[1], 8);
+    mbar_init(&p_ready[0], 4 * G);
+    mbar_init(&p_ready[1], 4 * G);
+    mbar_init(&pv_done[0], 1);
+    mbar_init(&pv_done[1], 1);
+    mbar_init(o_free, 4 * G);
+    mbar_init(&s_free[0], 4 * G);
+    mbar_init(&s_free[1], 4 * G);
     mbar_init(&drain[0], 1);
     mbar_init(&drain[1], 1);
     *abort_flag = 0;
@@ -697,7 +709,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
       }
       __syncwarp();
     }
-  } else if (warp == 10) {
+  } else if (warp == 2 + 4 * G) {
     // ------------------------------------------------------ O^T += V^T P^T
     // A warp of its own: S^T of a later tile and PV of this one become ready in
     // either order, and neither waits behind the other.
@@ -705,18 +717,18 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
       constexpr uint32_t I_O = idesc_bf16_f32(128, N, 1, 1);     // both read MN-major
       const uint32_t lead = elect_lead();
       Ring vr(pl.slots);
-      const uint32_t p_lo = desc_mn<CHUNK>(smem0 + pl.off_p);
       uint32_t g = 0, items = 0;
       bool ok = true, issued = false;
       for (PagedWalk<N, KT> w(rg, H, total, count, b_0, rt_0, tile_0); w.ok() && ok; w.next(), ++items) {
         for (int t = w.t0; t < w.t1 && ok; ++t, ++g) {
-          ok = pa_wait(p_ready, g & 1u, abort_flag, status, DSV3_ERR_WAIT_FULL);
+          ok = pa_wait(&p_ready[g & 1u], (g >> 1) & 1u, abort_flag, status, DSV3_ERR_WAIT_FULL);
           // the last item's O^T has been read out
           if (ok && t == w.t0 && items > 0)
             ok = pa_wait(o_free, (items - 1) & 1u, abort_flag, status, DSV3_ERR_WAIT_TMEM);
           if (!ok) break;
           tc_fence_after();
           const uint32_t acc = t > w.t0;
+          const uint32_t p_lo = desc_mn<CHUNK>(smem0 + pl.off_p + (g & 1u) * (pl.pbufs - 1) * PBUF);
           for (int m = 0; m < pl.LP; ++m) {
             const uint32_t v_lo = desc_mn<CHUNK>(smem0 + vr.slot * PAIR), d = tmem + (2 + m) * N;
             umma_lead(lead, d, v_lo, p_lo, kPaDescHi, I_O, acc);
@@ -726,7 +738,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
             commit_lead(lead, &pair_empty[vr.slot]);
             vr.next();
           }
-          commit_lead(lead, pv_done);
+          commit_lead(lead, &pv_done[g & 1u]);
           issued = true;
         }
       }
@@ -742,15 +754,15 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
     const int quarter = warp & 3;                  // TMEM lanes 32 * quarter ..
     // A key tile of 64 fills 16 TMEM lanes of each quarter; the two half warps
     // then take different columns of the same 16 keys.
-    constexpr int NC = KT == 64 ? N / 4 : N / 2;   // score columns of a thread
+    constexpr int NH = N / G;                      // rows of a warpgroup
+    constexpr int NC = KT == 64 ? NH / 2 : NH;     // rows of a thread
     constexpr int L = KT == 64 ? 16 : 32;          // lanes that hold different keys
-    constexpr int NH = N / 2;                      // columns of a half
     const int group = KT == 64 ? lane >> 4 : 0;
     const int key = quarter * L + (lane & (L - 1));
     const int ht = (warp - 2 - 4 * half) * 32 + lane;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const int col0 = half * NH + group * NC;
-    float* myred = red + half * 128;               // [32][4]
+    float* myred = red + half * NH * 4;            // [NH][4]
     float4* mref4 = reinterpret_cast<float4*>(mref + col0);
     const int4* lim4 = reinterpret_cast<const int4*>(lim + col0);
     uint32_t g = 0;
@@ -857,7 +869,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
             l[c + 3] *= f.w;
           }
           if (t > w.t0) {   // the first tile of an item overwrites O^T
-            pa_wait(pv_done, (g - 1) & 1u, abort_flag, status, DSV3_ERR_WAIT_TMEM);
+            pa_wait(&pv_done[(g - 1) & 1u], ((g - 1) >> 1) & 1u, abort_flag, status, DSV3_ERR_WAIT_TMEM);
             tc_fence_after();
 #pragma unroll 1
             for (int i = 0; i < pl.LP * (NH / 8); ++i) {
@@ -877,9 +889,12 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_free[g & 1u]);
-        // P and O^T of the previous tile are no longer in use by the tensor core
-        if (g > 0) pa_wait(pv_done, (g - 1) & 1u, abort_flag, status, DSV3_ERR_WAIT_TMEM);
-        uint8_t* prow = smem + pl.off_p + key * 128;
+        // the tile that last used this P buffer is through
+        if (g >= (uint32_t)pl.pbufs) {
+          const uint32_t u = g - pl.pbufs;
+          pa_wait(&pv_done[u & 1u], (u >> 1) & 1u, abort_flag, status, DSV3_ERR_WAIT_TMEM);
+        }
+        uint8_t* prow = smem + pl.off_p + (g & 1u) * (pl.pbufs - 1) * PBUF + key * 128;
         if constexpr (NC == 4) {
           *reinterpret_cast<uint2*>(prow + (((col0 >> 3) ^ (key & 7)) << 4) + (col0 & 4) * 2) = make_uint2(pk[0], pk[1]);
         } else {
@@ -893,7 +908,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
         // rows of the pages past the cached length hold anything: zero them, so
         // that their zero weights do not meet an infinity or NaN
         if (t * KT + KT > w.s.len && pos >= w.s.len) {
-          for (int c = KT == 64 ? half * 2 + group : half; c < 2 * pl.LP; c += KT == 64 ? 4 : 2) {
+          for (int c = KT == 64 ? half * 2 + group : half; c < 2 * pl.LP; c += KT == 64 ? 2 * G : G) {
             const int slot = (g * pl.LP + (c >> 1)) % pl.slots;
             uint4* z = reinterpret_cast<uint4*>(smem + slot * PAIR + (c & 1) * CHUNK + key * 128);
 #pragma unroll
@@ -903,7 +918,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
         fence_proxy_async_smem();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_ready);
+        if (lane == 0) mbar_arrive(&p_ready[g & 1u]);
         // row sums over the rounded weights, while the tensor core runs
 #pragma unroll
         for (int c = 0; c < NC; c += 2) {
@@ -912,7 +927,7 @@ __global__ void __launch_bounds__(kPaThreads, 1) paged_attention_tc_kernel(
         }
       }
       // ---- item epilogue
-      pa_wait(pv_done, (g - 1) & 1u, abort_flag, status, DSV3_ERR_WAIT_TMEM);
+      pa_wait(&pv_done[(g - 1) & 1u], ((g - 1) >> 1) & 1u, abort_flag, status, DSV3_ERR_WAIT_TMEM);
       tc_fence_after();
       const bool whole = w.t0 == 0 && w.t1 == w.nt;
       const int slot = 2 * blockIdx.x + (w.t0 == 0 ? 1 : 0);
