@@ -277,6 +277,58 @@ class InferenceEngine:
         out = logits[:, :self.V].view(B, S, self.V)
         return out, (x.view(B, S, self.D) if want_hidden else None)
 
+    # --------------------------------------------------------- paged cache
+    def _absorbed_rows(self, attn):
+        """``[H * (R + dr), Din]``: each head's rows of ``Wq_lat`` followed by its rows of ``Wq_pe``."""
+        wq_lat, wq_pe, _ = self._absorbed(attn)
+        k = self._key("absrows", self._wq(attn), attn.wkv_b.weight)
+        got = self._cache.get(k)
+        if got is None:
+            self._drop("absrows", self._wq(attn))
+            got = torch.cat([wq_lat.view(self.H, self.R, -1), wq_pe.view(self.H, self.dr, -1)], 1)
+            got = got.reshape(self.H * (self.R + self.dr), -1).contiguous()
+            self._cache[k] = got
+        return got
+
+    def _attn_paged(self, attn, xn, pages, table, cu, lens, pos, out):
+        """Absorbed attention of a ragged batch of new tokens over one layer's pages."""
+        C, T, W = self.C, xn.shape[0], self.R + self.dr
+        kv_a = self._lin(xn, self.bf16(attn.wkv_a.weight))
+        C.latent_cache_append(pages, kv_a, attn.kv_norm.weight.detach().float().contiguous(), self.cos, self.sin, table,
+                              cu, lens, 1e-6)
+        q = self._lin(self._q_input(attn, xn), self._absorbed_rows(attn)).view(T, self.H, W)
+        C.rope_inplace(q, self.R, self.dr // 2, self.cos, self.sin, pos, 1, 0, False)
+        o_lat = C.paged_latent_attention(q, pages, table, cu, lens, self.R, attn.softmax_scale)
+        C.linear_fwd(o_lat.view(T, self.H * self.R), self._absorbed(attn)[2], out, True)
+
+    @torch.no_grad()
+    def forward_paged(self, tokens: torch.Tensor, cache, block_table: torch.Tensor, cu_seqlens: torch.Tensor,
+                      seq_lens: torch.Tensor) -> torch.Tensor:
+        """Logits ``[B, V]`` (bf16) after the last new token of each sequence.
+
+        ``tokens [T]`` are the new tokens of a ragged batch over the paged cache
+        ``cache`` (``ops.paged``: any mix of prompts, chunks of prompts and single
+        tokens), whose rows are written first.
+        """
+        from .paged import token_positions
+        m, C = self.model, self.C
+        T = tokens.numel()
+        pos = token_positions(cu_seqlens, seq_lens, T)[1].to(torch.int32)
+        x = torch.empty(T, self.D, dtype=F32, device=self.device)
+        C.embedding_fwd(tokens.reshape(-1).long().contiguous(), m.embed.weight.detach().float().contiguous(), x)
+        for i, layer in enumerate(m.layers):
+            self._attn_paged(layer.attn, self._norm(x, layer.attn_norm.weight), cache.pages[i], block_table, cu_seqlens,
+                             seq_lens, pos, x)
+            xn = self._norm(x, layer.ffn_norm.weight)
+            if hasattr(layer.ffn, "experts"):
+                self._moe(layer.ffn, xn, x)
+            else:
+                self._dense_ffn(layer.ffn.w1.weight, layer.ffn.w3.weight, layer.ffn.w2.weight, xn, x)
+        x = x[(cu_seqlens[1:].long() - 1).clamp(min=0)]
+        logits = torch.empty(x.shape[0], self.Vp, dtype=BF16, device=self.device)
+        C.linear_fwd(self._norm(x, m.norm.weight), self.bf16(m.head.weight), logits[:, :self.V])
+        return logits[:, :self.V]
+
     # ------------------------------------------------------- graph decode
     def _graph_key(self, B: int) -> tuple:
         m = self.model

@@ -26,8 +26,11 @@ below.  On CUDA a page or position out of range is skipped and reported by
 """
 from __future__ import annotations
 
+from typing import List
+
 import torch
 
+from . import norm as norm_ops
 from ._ext import native
 
 
@@ -35,7 +38,7 @@ def token_positions(cu_seqlens: torch.Tensor, seq_lens: torch.Tensor, total: int
     """``(sequence, position)`` of each of ``total`` new tokens (int64)."""
     t = torch.arange(total, device=cu_seqlens.device)
     seq = torch.searchsorted(cu_seqlens[1:].long().contiguous(), t, right=True)
-    if total and int(seq[-1]) >= seq_lens.numel():
+    if total and not seq.is_cuda and int(seq[-1]) >= seq_lens.numel():
         raise IndexError(f"cu_seqlens covers {int(cu_seqlens[-1])} of {total} tokens")
     return seq, seq_lens.long()[seq] - cu_seqlens.long()[seq + 1] + t
 
@@ -92,3 +95,70 @@ def paged_latent_attention(q: torch.Tensor, pages: torch.Tensor, block_table: to
         p = torch.where((pos >= 0)[:, None, None], s.softmax(dim=-1), torch.zeros_like(s))
         out[lo:hi] = torch.einsum("thj,jr->thr", p, kv[:, :kv_rank]).to(q.dtype)
     return out
+
+
+class PagedLatentCache:
+    """Pages of the latent cache of every layer, and a host-side list of free ones.
+
+    ``pages [layers, pool, page, R + dr]``; ``take`` and ``give`` hand page ids
+    out and back (the caller writes them into its block tables).  One id stands
+    for the same page in every layer.
+    """
+
+    def __init__(self, config: dict, pool: int, page_size: int = 64, device=None, dtype=torch.bfloat16):
+        if page_size < 8 or page_size > 256 or page_size & (page_size - 1):
+            raise ValueError(f"page_size must be a power of two from 8 to 256, got {page_size}")
+        self.page_size = page_size
+        width = config["kv_lora_rank"] + config["qk_rope_head_dim"]
+        self.pages = torch.empty(config["n_layers"], pool, page_size, width, device=device, dtype=dtype)
+        self._free: List[int] = list(range(pool - 1, -1, -1))
+
+    @property
+    def free(self) -> int:
+        """Number of pages that are not handed out."""
+        return len(self._free)
+
+    def take(self, n: int) -> List[int]:
+        """``n`` page ids; raises ``RuntimeError`` if fewer are free."""
+        if n > len(self._free):
+            raise RuntimeError(f"paged cache: {n} pages wanted, {len(self._free)} of {self.pages.shape[1]} free")
+        return [self._free.pop() for _ in range(n)]
+
+    def give(self, ids: List[int]) -> None:
+        """Return pages that ``take`` handed out."""
+        self._free.extend(ids)
+
+
+@torch.no_grad()
+def paged_step(model, tokens: torch.Tensor, cache: PagedLatentCache, block_table: torch.Tensor,
+               cu_seqlens: torch.Tensor, seq_lens: torch.Tensor) -> torch.Tensor:
+    """Run the new ``tokens [T]`` of a ragged batch through the model.
+
+    Writes their cache rows and returns the logits after the last new token of
+    each sequence, ``[B, vocab]`` (a sequence without new tokens gets an
+    unspecified row).  Metadata as above.
+    """
+    if tokens.is_cuda:
+        return model.native_inference().forward_paged(tokens, cache, block_table, cu_seqlens, seq_lens)
+    from .decode import _row_rope
+    from .rope import rope_cos_sin
+    cfg = model.config
+    cos, sin = rope_cos_sin(cfg["max_seq_len"], cfg["qk_rope_head_dim"], float(cfg["rope_theta"]))
+    _, pos = token_positions(cu_seqlens, seq_lens, tokens.numel())
+    h = model.embed(tokens.long()).unsqueeze(1)                                    # [T, 1, dim]
+    for i, layer in enumerate(model.layers):
+        attn = layer.attn
+        x = norm_ops.rms_norm(h, layer.attn_norm.weight, layer.attn_norm.eps)
+        attn._extend_rope(attn.max_seq_len, x.device)
+        latent_cache_append(cache.pages[i], attn.wkv_a(x)[:, 0], attn.kv_norm.weight, cos, sin, block_table, cu_seqlens,
+                            seq_lens)
+        q_nope, q_pe = attn._queries(x)
+        q_pe = _row_rope(q_pe, attn.freqs_cis[pos])
+        w_k, w_v = attn._wkv_b_split()
+        q = torch.cat([torch.einsum("thd,hdr->thr", q_nope[:, 0], w_k), q_pe[:, 0]], dim=-1)
+        o = paged_latent_attention(q, cache.pages[i], block_table, cu_seqlens, seq_lens, attn.kv_lora_rank,
+                                   attn.softmax_scale)
+        h = h + attn.wo(torch.einsum("thr,hdr->thd", o, w_v).reshape(tokens.numel(), 1, -1))
+        h = h + layer.ffn(norm_ops.rms_norm(h, layer.ffn_norm.weight, layer.ffn_norm.eps))
+    last = (cu_seqlens[1:].long() - 1).clamp(min=0)
+    return model.head(model.final_hidden(h[last, 0]))
