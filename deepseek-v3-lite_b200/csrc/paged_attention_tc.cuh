@@ -2,16 +2,20 @@
 // Included by paged.cu inside its anonymous namespace, after Ragged.
 //
 // The rows of sequence b are its (token, head) pairs, n_b * H of them, cut
-// into row tiles of N; a key tile is 128 cached rows.  Both products are
-// computed transposed, so that the cached rows are the 128-wide M side of the
-// first and the latent columns the M side of the second, and one copy of a key
-// tile in shared memory serves both:
+// into row tiles of N; a key tile is KT cached rows.  Both products are
+// computed transposed, so that the cached rows are the M side of the first and
+// the latent columns the M side of the second, and one copy of a key tile in
+// shared memory serves both:
 //
-//   S^T [128 keys x N rows] = K [128 x D] . Q^T                 (K-major A)
+//   S^T [KT keys x N rows] = K [KT x D] . Q^T                   (K-major A)
 //   P^T = 2^(scale log2(e) S^T - m)                             (bf16, [key][row])
-//   O^T [R x N rows]       += V^T [R x 128 keys] . P^T          (the same K, read MN-major)
+//   O^T [R x N rows]      += V^T [R x KT keys] . P^T            (the same K, read MN-major)
 //
-// The cache row [latent | rotated key] is read as 64-column chunks [128 x 64]
+// KT is 64: with R 512 and N 64 the shared memory then holds two key tiles (128
+// rows left no room for a second; 441 us against 361 us for 4 x 512 new tokens),
+// and an MMA of 64 keys and 64 rows takes 32 cycles against 48 of 128 keys.
+//
+// The cache row [latent | rotated key] is read as 64-column chunks [KT x 64]
 // with a 128-byte swizzle; chunk pairs 0 .. LP-1 cover the latent (LP =
 // ceil(R / 128)), and where D reaches past them one more tail chunk holds the
 // rest of the rotated key.  Columns past D are zero-filled by TMA, rows past
@@ -1060,15 +1064,46 @@ __global__ void __launch_bounds__(FEW ? 512 : 256) paged_merge_kernel(const floa
     if (ml.y > 0.f) M = fmaxf(M, ml.x);
   }
   M = warp_max(M);
-  // threads of one part: R / 4 of them hold four latent columns each
-  const int tpp = FEW ? R / 4 : 32, groups = FEW ? 512 / tpp : 1, grp = FEW ? tid / tpp : 0;
-  if constexpr (FEW) {
+  if constexpr (!FEW) {
+    // a lane holds up to 4 x 4 latent columns: one pass over the parts, all loads
+    // of a part in flight together
+    float sum = 0.f;
+    float4 acc[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+    for (int i = 0; i < parts; ++i) {
+      const size_t k = at(i);
+      const float2 ml = part_ml[k];
+      float4 o[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (lane * 4 + 128 * c < R) o[c] = *reinterpret_cast<const float4*>(part_o + k * R + lane * 4 + 128 * c);
+      const float wgt = ml.y == 0.f ? 0.f : ex2_approx(ml.x - M);
+      sum += ml.y * wgt;
+      if (wgt != 0.f) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          acc[c].x += o[c].x * wgt;
+          acc[c].y += o[c].y * wgt;
+          acc[c].z += o[c].z * wgt;
+          acc[c].w += o[c].w * wgt;
+        }
+      }
+    }
+    const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (lane * 4 + 128 * c < R)
+        *reinterpret_cast<uint2*>(out + (size_t)(rc.x + n) * R + lane * 4 + 128 * c) =
+            make_uint2(pack_bf16x2(acc[c].x * inv, acc[c].y * inv), pack_bf16x2(acc[c].z * inv, acc[c].w * inv));
+  } else {
+    // R / 4 threads of a part hold four latent columns each; the parts of a thread
+    // group are added first, then the groups in order
     if (lane == 0) s_m[warp] = M;
     __syncthreads();
-    M = s_m[lane & 15];
-    M = warp_max(M);
-  }
-  for (int r = FEW ? (tid % tpp) * 4 : lane * 4; r < R; r += FEW ? R : 128) {
+    M = warp_max(s_m[lane & 15]);
+    const int tpp = R / 4, groups = 512 / tpp, grp = tid / tpp, r = (tid % tpp) * 4;
     float sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     if (grp < groups) {
@@ -1087,24 +1122,20 @@ __global__ void __launch_bounds__(FEW ? 512 : 256) paged_merge_kernel(const floa
         }
       }
     }
-    if constexpr (FEW) {
-      s_acc[tid] = acc;
-      if (tid % tpp == 0 && grp < groups) s_sum[grp] = sum;
-      __syncthreads();
-      if (grp > 0) return;
-      for (int i = 1; i < groups; ++i) {
-        const float4 o = s_acc[i * tpp + tid];
-        acc.x += o.x;
-        acc.y += o.y;
-        acc.z += o.z;
-        acc.w += o.w;
-        sum += s_sum[i];
-      }
+    s_acc[tid] = acc;
+    if (tid % tpp == 0 && grp < groups) s_sum[grp] = sum;
+    __syncthreads();
+    if (grp > 0) return;
+    for (int i = 1; i < groups; ++i) {
+      const float4 o = s_acc[i * tpp + tid];
+      acc.x += o.x;
+      acc.y += o.y;
+      acc.z += o.z;
+      acc.w += o.w;
+      sum += s_sum[i];
     }
     const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
-    uint2 v;
-    v.x = pack_bf16x2(acc.x * inv, acc.y * inv);
-    v.y = pack_bf16x2(acc.z * inv, acc.w * inv);
-    *reinterpret_cast<uint2*>(out + (size_t)(rc.x + n) * R + r) = v;
+    *reinterpret_cast<uint2*>(out + (size_t)(rc.x + n) * R + r) =
+        make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
   }
 }
