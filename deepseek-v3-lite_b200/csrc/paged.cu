@@ -293,9 +293,8 @@ at::Tensor paged_latent_attention(const at::Tensor& q, const at::Tensor& pages, 
   // fit in TMEM and the sequences fill it.
   const int64_t rows = (T * H + rg.B - 1) / rg.B;
   const int N = rows <= 16 ? 16 : rows <= 32 && T == rg.B ? 32 : rows <= 64 || R > 256 ? 64 : 128;
-  constexpr int KT = 64;
   PagedPlan pl;
-  TORCH_CHECK(paged_plan(N, KT, (int)R, (int)D, pl), op, ": no shared-memory plan");
+  TORCH_CHECK(paged_plan(N, (int)R, (int)D, pl), op, ": no shared-memory plan");
   auto work = at::Tensor(
       at::detail::empty_cuda({sms * (2 * N * (R + 2) + 4)}, at::kFloat, pages.device(), c10::nullopt));
   int4* rec = reinterpret_cast<int4*>(work.data_ptr<float>());
@@ -314,11 +313,11 @@ at::Tensor paged_latent_attention(const at::Tensor& q, const at::Tensor& pages, 
   bf16* o = reinterpret_cast<bf16*>(out.data_ptr());
   static std::atomic<uint64_t> opted[4];   // devices on which each variant may take all shared memory
   const int variant = N == 16 ? 0 : N == 32 ? 1 : N == 64 ? 2 : 3;
-#define DSV3_PAGED(N_, KT_)                                                                                           \
+#define DSV3_PAGED(N_)                                                                                           \
   do {                                                                                                           \
-    allow_shared_memory(paged_attention_tc_kernel<N_, KT_>, opted[variant]);                                      \
-    paged_attention_tc_kernel<N_, KT_><<<sms, pa_threads(N_), pl.smem, st>>>(                                             \
-        tm_q, tm_kv, pl, rg, (int)T, (int)H, (int)R, (int)D, (float)(scale * 1.4426950408889634), 1, o, part, ml, \
+    allow_shared_memory(paged_attention_tc_kernel<N_>, opted[variant]);                                      \
+    paged_attention_tc_kernel<N_><<<sms, pa_threads(N_), pl.smem, st>>>(                                             \
+        tm_q, tm_kv, pl, rg, (int)T, (int)H, (int)R, (int)D, (float)(scale * 1.4426950408889634), o, part, ml, \
         rec, status_ptr());                                                                                      \
     C10_CUDA_KERNEL_LAUNCH_CHECK();                                                                              \
     C10_CUDA_CHECK(few ? launch_dependent(paged_merge_kernel<N_, true>, dim3((unsigned)cuts, N_), 512, st,       \
@@ -326,10 +325,10 @@ at::Tensor paged_latent_attention(const at::Tensor& q, const at::Tensor& pages, 
                        : launch_dependent(paged_merge_kernel<N_, false>, dim3(sms, N_ / 8), 256, st,             \
                                           (const float*)part, (const float2*)ml, (const int4*)rec, sms, (int)R, o)); \
   } while (0)
-  if (N == 16) DSV3_PAGED(16, KT);
-  else if (N == 32) DSV3_PAGED(32, KT);
-  else if (N == 64) DSV3_PAGED(64, KT);
-  else DSV3_PAGED(128, KT);
+  if (N == 16) DSV3_PAGED(16);
+  else if (N == 32) DSV3_PAGED(32);
+  else if (N == 64) DSV3_PAGED(64);
+  else DSV3_PAGED(128);
 #undef DSV3_PAGED
   return out;
 }

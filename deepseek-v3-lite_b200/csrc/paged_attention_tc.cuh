@@ -22,12 +22,12 @@
 // the cached length are masked in S and zeroed in shared memory before the
 // second product (pages are never assumed to be initialised past that).
 //
-// A softmax thread owns one key and N / 2 of the rows: there is no per-row
+// A softmax thread owns one key and a few of the rows: there is no per-row
 // maximum over keys at hand, and none is needed.  Each row keeps a reference m
 // that any score may exceed by up to 2^8 without harm (sums and O are fp32, P
-// has the same relative precision at any scale); the 128 threads of a column
-// half vote per tile, and only when one exceeds it are the column maxima
-// computed, m moved and O^T rescaled.  Row sums are kept per thread and added
+// has the same relative precision at any scale); the 128 threads of a warpgroup
+// vote per tile, and only when one exceeds it are the rows' maxima computed, m
+// moved and O^T rescaled.  Row sums are kept per thread and added
 // up once per item, over the bf16-rounded P that the second product uses, so
 // that a row's weights sum to one exactly.
 //
@@ -43,12 +43,21 @@
 // and epilogue, and one warp for the second product.  Every wait is
 // bounded; after one ran out the softmax warps go on without waiting, so that
 // they meet at their barriers, and the others stop.
+//
+// Measured (R 512, 16 heads, pages of 64): 64 requests with 512 to 4,096 rows, one
+// token each, 39 us without the merge (169 MB, floor 26 us); two of 100,000 rows
+// 60 us (floor 42 us); 4 x 512 new tokens on 3,000 to 4,096 rows 361 us, 650
+// TFLOP/s: both products read their operands from shared memory at its full rate,
+// and TMA writes the key tiles into it as well (2,600 of the 3,300 cycles of a
+// tile).  R 192, 16 ragged chunks of up to 509 tokens: 78 us, bound by the softmax
+// and by the turn from one row tile to the next.
 
 // Softmax warpgroups of a row tile, each with its share of the rows: two for few
-// rows; four for 64 and 128, where two spent longer on a tile than the tensor core
-// (2,200 cycles against 1,400 for 128 rows).
+// rows; four for 64 and 128, where the softmax of a tile takes longer than its MMAs
+// (2,200 cycles against 1,400 for 128 rows of R 192, with two).
 constexpr int pa_groups(int N) { return N >= 64 ? 4 : 2; }
 constexpr int pa_threads(int N) { return 32 * (3 + 4 * pa_groups(N)); }   // TMA, S, softmax, PV
+constexpr int KT = 64;                       // key tile
 constexpr int kPaMaxSlots = 16;
 constexpr int kPaSmem = 232448;              // shared memory of a CTA, at most
 constexpr float kPaUnset = -1e30f;           // reference of a row that has seen no key
@@ -64,7 +73,7 @@ struct PagedPlan {
 // Shared memory of a plan: ring | tail slots | P | Q | misc, with as many ring
 // slots as fit; at least two key tiles' worth, so that one loads while the
 // other is in use.
-inline bool paged_plan(int N, int KT, int R, int D, PagedPlan& p) {
+inline bool paged_plan(int N, int R, int D, PagedPlan& p) {
   const int chunk = KT * 128;
   p.LP = (R + 127) / 128;
   p.nch = (D + 63) / 64;
@@ -139,7 +148,7 @@ __device__ __forceinline__ int warp_uniform(int x) { return __shfl_sync(0xffffff
 
 // Key tiles of row tile rt: up to the position of its last row, at least one
 // (a row that sees nothing is still written).
-template <int N, int KT>
+template <int N>
 __device__ __forceinline__ int paged_key_tiles(const PagedSeq& s, int rt, int H) {
   const int last = min((rt + 1) * N, s.rows) - 1;
   const int keys = s.len - s.n + last / H + 1;
@@ -147,14 +156,14 @@ __device__ __forceinline__ int paged_key_tiles(const PagedSeq& s, int rt, int H)
 }
 
 // Key tiles of row tiles 0 .. k-1.
-template <int N, int KT>
+template <int N>
 __device__ __forceinline__ long long paged_tiles_before(const PagedSeq& s, int k, int H) {
   if (k <= 0) return 0;
   long long ans = 0;
   int full = k;
   if (k == s.tiles) {         // the last row tile may be short
     full = k - 1;
-    ans = paged_key_tiles<N, KT>(s, k - 1, H);
+    ans = paged_key_tiles<N>(s, k - 1, H);
   }
   // row tile i ends at row x = (i + 1) N - 1, at position p = len - n + x / H:
   // p / KT + 1 = ((len - n) H + x) / (KT H) + 1 tiles, one where p < 0
@@ -168,7 +177,7 @@ __device__ __forceinline__ long long paged_tiles_before(const PagedSeq& s, int k
 }
 
 // A CTA's share as a walk over items: (sequence, row tile, key tiles t0 .. t1).
-template <int N, int KT>
+template <int N>
 struct PagedWalk {
   const Ragged& r;
   int H, total;
@@ -179,7 +188,7 @@ struct PagedWalk {
       : r(r_), H(H_), total(total_), left(count), b(b0), rt(rt0), t0(tile0) {
     if (left > 0) {
       load();
-      nt = paged_key_tiles<N, KT>(s, rt, H);
+      nt = paged_key_tiles<N>(s, rt, H);
       t1 = min(nt, t0 + left);
     }
   }
@@ -206,7 +215,7 @@ struct PagedWalk {
         load();
       } while (s.tiles == 0);
     }
-    nt = paged_key_tiles<N, KT>(s, rt, H);
+    nt = paged_key_tiles<N>(s, rt, H);
     t1 = min(nt, left);
   }
 };
@@ -255,15 +264,8 @@ __device__ __forceinline__ void tmem_ld_half(uint32_t taddr, uint32_t* r) {
           : "r"(taddr + i), "n"(SPLIT));
   }
 }
-// W columns of S^T of this thread's key, at column c of its group.
-template <int KT, int NC, int W>
-__device__ __forceinline__ void ld_scores(uint32_t taddr, uint32_t (&r)[W]) {
-  if constexpr (KT == 64) tmem_ld_half<NC, W>(taddr, r);
-  else tmem_ld_cols<W>(taddr, r);
-}
-
-// Barrier of the 128 threads of one column half, with the OR of a predicate.
-__device__ __forceinline__ bool half_any(int half, bool v) {
+// Barrier of the 128 threads of a softmax warpgroup, with the OR of a predicate.
+__device__ __forceinline__ bool wg_any(int wg, bool v) {
   uint32_t out;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
@@ -271,12 +273,12 @@ __device__ __forceinline__ bool half_any(int half, bool v) {
       "barrier.cta.red.or.pred p, %2, 128, q;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(out)
-      : "r"((uint32_t)v), "r"(half + 1)
+      : "r"((uint32_t)v), "r"(wg + 1)
       : "memory");
   return out != 0;
 }
-__device__ __forceinline__ void half_sync(int half) {
-  asm volatile("barrier.cta.sync %0, 128;" ::"r"(half + 1) : "memory");
+__device__ __forceinline__ void wg_sync(int wg) {
+  asm volatile("barrier.cta.sync %0, 128;" ::"r"(wg + 1) : "memory");
 }
 
 __device__ __forceinline__ uint32_t float_key(float x) {
@@ -296,8 +298,9 @@ struct PagedStart {
   int b, rt, tile, found;
 };
 
-template <int N, int KT>
-__device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, int min_share, PagedStart* out, int* scan, unsigned int* status) {
+template <int N>
+__device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, PagedStart* out, int* scan,
+                                           unsigned int* status) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int THREADS = pa_threads(N), NW = THREADS / 32;
   // round 0 adds up all sequences; round 1 finds the one that holds the share's
@@ -314,7 +317,7 @@ __device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, in
         t = 0;
         if (b < r.B) {
           s = paged_seq<N>(r, b, H, total);
-          t = (int)paged_tiles_before<N, KT>(s, s.tiles, H);
+          t = (int)paged_tiles_before<N>(s, s.tiles, H);
           if (round == 0 && blockIdx.x == 0) {
             const int c0 = __ldg(r.cu + b), c1 = __ldg(r.cu + b + 1);
             if (__ldg(r.lens + b) > r.cols * r.page || c1 > total || c1 < c0 || (b == 0 && c0 != 0) ||
@@ -351,7 +354,6 @@ __device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, in
     }
     if (round == 0) {
       int share = (base + gridDim.x - 1) / gridDim.x;
-      if (share < min_share) share = min_share;
       target = share * blockIdx.x;
       if (tid == 0) {
         out->share = share;
@@ -373,8 +375,8 @@ __device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, in
       const int step = (hi - lo + THREADS - 1) / THREADS, k = lo + tid * step;
       const int k1 = min(k + step, hi);
       if (k < hi) {
-        const long long at = paged_tiles_before<N, KT>(s, k, H);
-        if (at <= local && (k1 == s.tiles || local < paged_tiles_before<N, KT>(s, k1, H))) {
+        const long long at = paged_tiles_before<N>(s, k, H);
+        if (at <= local && (k1 == s.tiles || local < paged_tiles_before<N>(s, k1, H))) {
           out->rt = k;
           out->tile = (int)(local - at);
         }
@@ -430,8 +432,6 @@ __device__ __forceinline__ void commit_lead(uint32_t leader, uint64_t* bar) {
       "r"(smem_u32(bar))
       : "memory");
 }
-// The issuing lane.  It has to come from elect.sync: under `lane == 0` the
-// compiler wraps each MMA in a divergent branch (90 to 200 cycles apiece).
 // The TMA loads and barrier arrivals of the producer are issued the same way.
 __device__ __forceinline__ void expect_lead(uint32_t leader, uint64_t* bar, uint32_t bytes) {
   asm volatile(
@@ -461,6 +461,8 @@ __device__ __forceinline__ void tma_lead_3d(uint32_t leader, uint32_t dst, const
       "r"(dst), "l"(desc), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
+// The issuing lane.  It has to come from elect.sync: under `lane == 0` the
+// compiler wraps each MMA in a divergent branch (90 to 200 cycles apiece).
 __device__ __forceinline__ uint32_t elect_lead() {
   uint32_t r;
   asm volatile(
@@ -519,11 +521,11 @@ struct Ring {
   }
 };
 
-template <int N, int KT>
+template <int N>
 __global__ void __launch_bounds__(pa_threads(N), 1) paged_attention_tc_kernel(
     const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ PagedPlan pl,
     const __grid_constant__ Ragged rg,
-    int total, int H, int R, int D, float scale_log2, int min_share, bf16* __restrict__ out,
+    int total, int H, int R, int D, float scale_log2, bf16* __restrict__ out,
     float* __restrict__ part_o, float2* __restrict__ part_ml, int4* __restrict__ rec, unsigned int* status) {
   constexpr int G = pa_groups(N), PBUF = (N + 63) / 64 * KT * 128;
   constexpr int CHUNK = KT * 128, PAIR = 2 * CHUNK;  // [KT keys x 64 columns], two of them (bytes)
@@ -582,7 +584,7 @@ __global__ void __launch_bounds__(pa_threads(N), 1) paged_attention_tc_kernel(
     tmem_relinquish();
   }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  paged_find<N, KT>(rg, H, total, min_share, start, scan, status);
+  paged_find<N>(rg, H, total, start, scan, status);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -598,7 +600,7 @@ __global__ void __launch_bounds__(pa_threads(N), 1) paged_attention_tc_kernel(
     Ring pr(pl.slots), tr(pl.tail ? pl.tails : 1);
     uint32_t pu = 0, tu = 0, items = 0;      // pair uses, tail uses
     bool ok = true;
-    for (PagedWalk<N, KT> w(rg, H, total, count, b_0, rt_0, tile_0); w.ok() && ok; w.next()) {
+    for (PagedWalk<N> w(rg, H, total, count, b_0, rt_0, tile_0); w.ok() && ok; w.next()) {
       ok = pa_wait(q_empty, (items & 1u) ^ 1u, abort_flag, status, DSV3_ERR_WAIT_EMPTY);
       if (!ok) break;
       ++items;
@@ -659,7 +661,7 @@ __global__ void __launch_bounds__(pa_threads(N), 1) paged_attention_tc_kernel(
       Ring sr(pl.slots), tr(pl.tail ? pl.tails : 1);
       uint32_t g = 0, items = 0;
       bool ok = true, issued = false;
-      for (PagedWalk<N, KT> w(rg, H, total, count, b_0, rt_0, tile_0); w.ok() && ok; w.next(), ++items) {
+      for (PagedWalk<N> w(rg, H, total, count, b_0, rt_0, tile_0); w.ok() && ok; w.next(), ++items) {
         ok = pa_wait(q_full, items & 1u, abort_flag, status, DSV3_ERR_WAIT_FULL);
         for (int t = w.t0; t < w.t1 && ok; ++t, ++g) {
           // two S^T buffers: this one's last tile has been read
@@ -723,7 +725,7 @@ __global__ void __launch_bounds__(pa_threads(N), 1) paged_attention_tc_kernel(
       Ring vr(pl.slots);
       uint32_t g = 0, items = 0;
       bool ok = true, issued = false;
-      for (PagedWalk<N, KT> w(rg, H, total, count, b_0, rt_0, tile_0); w.ok() && ok; w.next(), ++items) {
+      for (PagedWalk<N> w(rg, H, total, count, b_0, rt_0, tile_0); w.ok() && ok; w.next(), ++items) {
         for (int t = w.t0; t < w.t1 && ok; ++t, ++g) {
           ok = pa_wait(&p_ready[g & 1u], (g >> 1) & 1u, abort_flag, status, DSV3_ERR_WAIT_FULL);
           // the last item's O^T has been read out
@@ -754,33 +756,33 @@ __global__ void __launch_bounds__(pa_threads(N), 1) paged_attention_tc_kernel(
     }
   } else {
     // ---------------------------------------------------- softmax / epilogue
-    const int half = (warp - 2) >> 2;              // columns half * NC ..
+    const int wg = (warp - 2) >> 2;              // its rows are wg * NH ..
     const int quarter = warp & 3;                  // TMEM lanes 32 * quarter ..
     // A key tile of 64 fills 16 TMEM lanes of each quarter; the two half warps
     // then take different columns of the same 16 keys.
     constexpr int NH = N / G;                      // rows of a warpgroup
-    constexpr int NC = KT == 64 ? NH / 2 : NH;     // rows of a thread
-    constexpr int L = KT == 64 ? 16 : 32;          // lanes that hold different keys
-    const int group = KT == 64 ? lane >> 4 : 0;
+    constexpr int NC = NH / 2;                     // rows of a thread
+    constexpr int L = 16;                          // lanes that hold different keys
+    const int side = lane >> 4;
     const int key = quarter * L + (lane & (L - 1));
-    const int ht = (warp - 2 - 4 * half) * 32 + lane;
+    const int ht = (warp - 2 - 4 * wg) * 32 + lane;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-    const int col0 = half * NH + group * NC;
-    float* myred = red + half * NH * 4;            // [NH][4]
+    const int col0 = wg * NH + side * NC;
+    float* myred = red + wg * NH * 4;            // [NH][4]
     float4* mref4 = reinterpret_cast<float4*>(mref + col0);
     const int4* lim4 = reinterpret_cast<const int4*>(lim + col0);
     uint32_t g = 0;
     int4 my_rec = make_int4(-1, 0, 0, 0);
-    for (PagedWalk<N, KT> w(rg, H, total, count, b_0, rt_0, tile_0); w.ok(); w.next()) {
+    for (PagedWalk<N> w(rg, H, total, count, b_0, rt_0, tile_0); w.ok(); w.next()) {
       const int base = w.s.len - w.s.n;
       const int nr = min(N, w.s.rows - w.rt * N);
-      half_sync(half);                             // the last item's references are read
+      wg_sync(wg);                             // the last item's references are read
       if (ht < NH) {
-        const int n = half * NH + ht;
+        const int n = wg * NH + ht;
         reinterpret_cast<uint32_t*>(corr)[n] = 0u;
         lim[n] = n < nr ? base + (w.rt * N + n) / H + 1 : 0;
       }
-      half_sync(half);
+      wg_sync(wg);
       const int seen_by_all = base + (w.rt * N) / H + 1;      // keys that every row sees
       float l[NC];
 #pragma unroll
@@ -789,7 +791,7 @@ __global__ void __launch_bounds__(pa_threads(N), 1) paged_attention_tc_kernel(
         pa_wait(&s_full[g & 1u], (g >> 1) & 1u, abort_flag, status, DSV3_ERR_WAIT_TMEM);
         tc_fence_after();
         uint32_t sr[NC];
-        ld_scores<KT, NC, NC>(tmem + lane_base + (g & 1u) * N + half * NH, sr);
+        tmem_ld_half<NC, NC>(tmem + lane_base + (g & 1u) * N + wg * NH, sr);
         tmem_ld_wait();
         const int pos = t * KT + key;
         if (t * KT + KT > seen_by_all) {
@@ -819,10 +821,10 @@ __global__ void __launch_bounds__(pa_threads(N), 1) paged_attention_tc_kernel(
               mref4[c / 4] = m4;
             }
           }
-          half_sync(half);
+          wg_sync(wg);
         }
         // p = 2^(s - m) at the present references; where one is passed by more
-        // than 2^8 the half moves them and computes p again
+        // than 2^8 the warpgroup moves them and computes p again
         uint32_t pk[NC / 2];
         for (int attempt = 0;; ++attempt) {
           float over = -INFINITY;
@@ -837,7 +839,7 @@ __global__ void __launch_bounds__(pa_threads(N), 1) paged_attention_tc_kernel(
             pk[c / 2] = pack_bf16x2(ex2_approx(d0), ex2_approx(d1));
             pk[c / 2 + 1] = pack_bf16x2(ex2_approx(d2), ex2_approx(d3));
           }
-          if (!half_any(half, over > 8.f) || attempt == 1) break;
+          if (!wg_any(wg, over > 8.f) || attempt == 1) break;
           // column maxima of the tile: S^T is read again in slices, so that this
           // rare path is a short loop (unrolled over registers it ran from
           // instruction-cache misses, 14,000 cycles)
@@ -846,7 +848,7 @@ __global__ void __launch_bounds__(pa_threads(N), 1) paged_attention_tc_kernel(
           for (int c0 = 0; c0 < NC; c0 += W) {
             uint32_t u[W];
             float v[W];
-            ld_scores<KT, NC, W>(tmem + lane_base + (g & 1u) * N + half * NH + c0, u);
+            tmem_ld_half<NC, W>(tmem + lane_base + (g & 1u) * N + wg * NH + c0, u);
             tmem_ld_wait();
 #pragma unroll
             for (int c = 0; c < W; ++c)
@@ -855,15 +857,15 @@ __global__ void __launch_bounds__(pa_threads(N), 1) paged_attention_tc_kernel(
             if (lane % (L / W) == 0)
               atomicMax(reinterpret_cast<unsigned int*>(corr) + col0 + c0 + (lane & (L - 1)) * W / L, float_key(top));
           }
-          half_sync(half);
+          wg_sync(wg);
           if (ht < NH) {
-            const int n = half * NH + ht;
+            const int n = wg * NH + ht;
             const float old = mref[n], top = float_unkey(reinterpret_cast<uint32_t*>(corr)[n]);
             const float now = fmaxf(old, top);
             mref[n] = now;
             corr[n] = ex2_approx(old - now);
           }
-          half_sync(half);
+          wg_sync(wg);
 #pragma unroll
           for (int c = 0; c < NC; c += 4) {
             const float4 f = *reinterpret_cast<const float4*>(corr + col0 + c);
@@ -877,7 +879,7 @@ __global__ void __launch_bounds__(pa_threads(N), 1) paged_attention_tc_kernel(
             tc_fence_after();
 #pragma unroll 1
             for (int i = 0; i < pl.LP * (NH / 8); ++i) {
-              const int m = i / (NH / 8), c = half * NH + i % (NH / 8) * 8;
+              const int m = i / (NH / 8), c = wg * NH + i % (NH / 8) * 8;
               uint32_t o[8];
               tmem_ld8(tmem + lane_base + (2 + m) * N + c, o);
               tmem_ld_wait();
@@ -887,8 +889,8 @@ __global__ void __launch_bounds__(pa_threads(N), 1) paged_attention_tc_kernel(
             }
             tmem_st_wait();
           }
-          half_sync(half);
-          if (ht < NH) reinterpret_cast<uint32_t*>(corr)[half * NH + ht] = 0u;
+          wg_sync(wg);
+          if (ht < NH) reinterpret_cast<uint32_t*>(corr)[wg * NH + ht] = 0u;
         }
         tc_fence_before();
         __syncwarp();
@@ -912,7 +914,7 @@ __global__ void __launch_bounds__(pa_threads(N), 1) paged_attention_tc_kernel(
         // rows of the pages past the cached length hold anything: zero them, so
         // that their zero weights do not meet an infinity or NaN
         if (t * KT + KT > w.s.len && pos >= w.s.len) {
-          for (int c = KT == 64 ? half * 2 + group : half; c < 2 * pl.LP; c += KT == 64 ? 2 * G : G) {
+          for (int c = wg * 2 + side; c < 2 * pl.LP; c += 2 * G) {
             const int slot = (g * pl.LP + (c >> 1)) % pl.slots;
             uint4* z = reinterpret_cast<uint4*>(smem + slot * PAIR + (c & 1) * CHUNK + key * 128);
 #pragma unroll
@@ -940,24 +942,23 @@ __global__ void __launch_bounds__(pa_threads(N), 1) paged_attention_tc_kernel(
         const int s0 = start->first + (count - w.left);
         my_rec = make_int4((int)row0, nr, (s0 + w.nt - 1) / start->share, 0);
       }
-      constexpr int WL = NC < L ? NC : L;            // columns of a group folded at a time
-      constexpr int GR = 32 / L;                     // groups of a half
+      constexpr int WL = NC < L ? NC : L;            // rows of a half warp folded at a time
 #pragma unroll
       for (int c0 = 0; c0 < NC; c0 += WL) {
         const float v = fold_columns<WL, L>(*reinterpret_cast<float(*)[WL]>(&l[c0]), lane,
                                             [](float x, float y) { return x + y; });
-        if (c0 > 0) half_sync(half);               // the last columns are read
-        if (lane % (L / WL) == 0) myred[(group * WL + (lane & (L - 1)) * WL / L) * 4 + (warp - 2 - 4 * half)] = v;
-        half_sync(half);
-        if (ht < GR * WL) {
+        if (c0 > 0) wg_sync(wg);               // the last columns are read
+        if (lane % (L / WL) == 0) myred[(side * WL + (lane & (L - 1)) * WL / L) * 4 + (warp - 2 - 4 * wg)] = v;
+        wg_sync(wg);
+        if (ht < 2 * WL) {
           const float4 r4 = *reinterpret_cast<const float4*>(myred + ht * 4);
           const float sum = (r4.x + r4.y) + (r4.z + r4.w);
-          const int n = half * NH + ht / WL * NC + c0 + ht % WL;
+          const int n = wg * NH + ht / WL * NC + c0 + ht % WL;
           if (!whole) part_ml[(size_t)slot * N + n] = make_float2(mref[n], sum);
           corr[n] = !whole ? 1.f : (sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum));
         }
       }
-      half_sync(half);
+      wg_sync(wg);
       constexpr int W = NH < 32 ? NH : 32;
       // O^T out: a thread holds one latent column of W rows; the warp turns eight
       // rows (four of fp32 partials) at a time into 16-byte stores in 512 bytes of
@@ -966,7 +967,7 @@ __global__ void __launch_bounds__(pa_threads(N), 1) paged_attention_tc_kernel(
       uint8_t* stage = smem + pl.off_p + (warp - 2) * 512;
 #pragma unroll 1
       for (int i = 0; i < pl.LP * (NH / W); ++i) {
-        const int m = i / (NH / W), n0 = half * NH + i % (NH / W) * W;
+        const int m = i / (NH / W), n0 = wg * NH + i % (NH / W) * W;
         const int r0 = 128 * m + quarter * 32;
         if (n0 >= nr || r0 >= R) continue;
         uint32_t o[W];
