@@ -150,6 +150,17 @@ def test_attention_strided_pool_and_table():
     assert torch.equal(paged_latent_attention(qt, pages, table, cu, lens, 512, 0.07), want)
 
 
+@pytest.mark.parametrize("heads,new", [(4, 1), (40, 1), (12, 12)])
+def test_attention_of_more_sequences_than_threads(heads, new):
+    """1,300 sequences of 0 to ``new`` tokens over 0 to 200 rows: the search for a share takes several rounds."""
+    from ops.paged import paged_latent_attention
+    g = torch.Generator().manual_seed(heads)
+    n = torch.randint(0 if new > 1 else 1, new + 1, (1300,), generator=g).tolist()
+    c = torch.randint(0, 200, (1300,), generator=g).tolist()
+    args = make([(a, max(a, b)) for a, b in zip(n, c)], heads, 64, 16, 32, seed=heads)
+    check(paged_latent_attention(*args, 64, 0.11), *oracle(*args, 64, 0.11))
+
+
 def test_attention_is_repeatable_on_any_stream():
     from ops.paged import paged_latent_attention
     args = make([(1, 5000), (200, 900), (3, 30)], 16, 512, 64, 64, seed=10)
