@@ -101,9 +101,11 @@ __global__ void rmsnorm_bwd_kernel(const TDy* __restrict__ dy, long lddy, const 
 // Rotate pairs (x[2i], x[2i+1]) of a [T, H, ...] bf16 tensor in place, at
 // column offset `off` of each head.  Position of token t is pos[t] when given,
 // else (t % seqlen) + start.  `inverse` rotates by -theta (backward pass).
+// Positions may come from a caller's metadata: one outside the tables' npos rows
+// is reported through the status word and its token left as it is.
 __global__ void rope_kernel(__nv_bfloat16* __restrict__ x, long ld_tok, long ld_head, int off, int T, int H,
-                            int half, const float* __restrict__ cosv, const float* __restrict__ sinv,
-                            const int* __restrict__ pos, int seqlen, int start, int inverse) {
+                            int half, const float* __restrict__ cosv, const float* __restrict__ sinv, int npos,
+                            const int* __restrict__ pos, int seqlen, int start, int inverse, unsigned int* status) {
   const long idx = (long)blockIdx.x * blockDim.x + threadIdx.x;
   const long total = (long)T * H * half;
   if (idx >= total) return;
@@ -111,6 +113,10 @@ __global__ void rope_kernel(__nv_bfloat16* __restrict__ x, long ld_tok, long ld_
   const int h = (idx / half) % H;
   const int t = idx / ((long)half * H);
   const int p = pos ? pos[t] : (t % seqlen) + start;
+  if (p < 0 || p >= npos) {
+    if (i == 0 && h == 0) record_error(status, DSV3_ERR_BOUNDS);
+    return;
+  }
   const float c = cosv[(size_t)p * half + i];
   const float s = inverse ? -sinv[(size_t)p * half + i] : sinv[(size_t)p * half + i];
   __nv_bfloat16* e = x + (size_t)t * ld_tok + (size_t)h * ld_head + off + 2 * i;
@@ -880,13 +886,18 @@ void rope_inplace(at::Tensor& x, int64_t off, int64_t half, const at::Tensor& co
                   c10::optional<at::Tensor> pos, int64_t seqlen, int64_t start, bool inverse) {
   // x: [T, H, W] bf16 view (any strides on T / H, unit on W)
   TORCH_CHECK(x.dim() == 3 && x.stride(2) == 1 && x.scalar_type() == at::kBFloat16, "rope_inplace: [T,H,W] bf16");
+  TORCH_CHECK(cosv.dim() == 2 && cosv.size(1) == half && sinv.sizes() == cosv.sizes() && cosv.is_contiguous() &&
+                  sinv.is_contiguous(),
+              "rope_inplace: cos and sin are contiguous tables [positions, half]");
+  TORCH_CHECK(!pos || (pos->scalar_type() == at::kInt && pos->is_contiguous() && pos->numel() >= x.size(0)),
+              "rope_inplace: pos is a contiguous int32 tensor of one position per token");
   const int T = x.size(0), H = x.size(1);
   const at::cuda::CUDAGuard guard(x.device());
   const long total = (long)T * H * half;
   rope_kernel<<<blocks_for(total, 256), 256, 0, at::cuda::getCurrentCUDAStream()>>>(
       reinterpret_cast<__nv_bfloat16*>(x.data_ptr()), x.stride(0), x.stride(1), off, T, H, half,
-      cosv.data_ptr<float>(), sinv.data_ptr<float>(), pos ? pos->data_ptr<int>() : nullptr, seqlen, start,
-      inverse ? 1 : 0);
+      cosv.data_ptr<float>(), sinv.data_ptr<float>(), (int)cosv.size(0), pos ? pos->data_ptr<int>() : nullptr, seqlen,
+      start, inverse ? 1 : 0, status_ptr());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
