@@ -15,6 +15,8 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <cfloat>
+
 #include "common.cuh"
 #include "status.h"
 
@@ -53,7 +55,10 @@ __global__ void __launch_bounds__(256) router_topk_kernel(const float* __restric
       if (e < E) {
         const float s = 1.0f / (1.0f + __expf(-logits[(size_t)t * ldl + e]));
         sc[i] = s;
-        bsc[i] = s + bias_l[i];
+        // a NaN score ranks below every number but above the experts already
+        // taken (-inf), so that k distinct ids in range are always found; the
+        // NaN itself stays in the weight
+        bsc[i] = fmaxf(s + bias_l[i], -FLT_MAX);
       } else {
         sc[i] = 0.f;
         bsc[i] = -INFINITY;
