@@ -296,6 +296,7 @@ struct PagedStart {
   int first;                  // flat index of its first key tile
   int local;                  // its index within sequence b
   int b, rt, tile, found;
+  int gap;                    // the offsets do not cover every token once
 };
 
 template <int N>
@@ -303,6 +304,7 @@ __device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, Pa
                                            unsigned int* status) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int THREADS = pa_threads(N), NW = THREADS / 32;
+  if (tid == 0) out->gap = 0;
   // round 0 adds up all sequences; round 1 finds the one that holds the share's
   // first tile (a batch of up to THREADS sequences is still in registers)
   int target = 0, t = 0;
@@ -312,17 +314,17 @@ __device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, Pa
     int base = 0;
     for (int b0 = 0; b0 < r.B; b0 += THREADS) {
       const int b = b0 + tid;
+      bool gap = false;
       if (round == 0 || r.B > THREADS) {
         s.tiles = 0;
         t = 0;
         if (b < r.B) {
           s = paged_seq<N>(r, b, H, total);
           t = (int)paged_tiles_before<N>(s, s.tiles, H);
-          if (round == 0 && blockIdx.x == 0) {
+          if (round == 0) {
             const int c0 = __ldg(r.cu + b), c1 = __ldg(r.cu + b + 1);
-            if (__ldg(r.lens + b) > r.cols * r.page || c1 > total || c1 < c0 || (b == 0 && c0 != 0) ||
-                (b == r.B - 1 && c1 != total))
-              record_error(status, DSV3_ERR_BOUNDS);
+            gap = c1 > total || c1 < c0 || (b == 0 && c0 != 0) || (b == r.B - 1 && c1 != total);
+            if (blockIdx.x == 0 && (gap || __ldg(r.lens + b) > r.cols * r.page)) record_error(status, DSV3_ERR_BOUNDS);
           }
         }
       }
@@ -334,6 +336,7 @@ __device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, Pa
       }
       if (lane == 31) scan[warp] = inc;
       __syncthreads();
+      if (gap) out->gap = 1;
       int before = base, all = base;
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
@@ -386,6 +389,24 @@ __device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, Pa
       hi = step > 1 ? min(lo + step, hi) : lo;
       __syncthreads();
     }
+  }
+}
+
+// Zeroes the result of the tokens that no sequence holds; the whole CTA, a token
+// per CTA in turn.  Only for offsets that are reported as wrong.
+__device__ __forceinline__ void paged_clear_gaps(const Ragged& r, int total, size_t row_bytes, uint8_t* out) {
+#pragma unroll 1
+  for (int t = blockIdx.x; t < total; t += gridDim.x) {
+    bool held = false;
+#pragma unroll 1
+    for (int b = threadIdx.x; b < r.B; b += blockDim.x) {
+      const int c0 = __ldg(r.cu + b), c1 = __ldg(r.cu + b + 1);
+      held |= c0 >= 0 && c1 <= total && c0 <= t && t < c1;
+    }
+    if (__syncthreads_or(held)) continue;
+#pragma unroll 1
+    for (size_t i = threadIdx.x * 16; i < row_bytes; i += blockDim.x * 16)
+      *reinterpret_cast<uint4*>(out + t * row_bytes + i) = make_uint4(0, 0, 0, 0);
   }
 }
 
@@ -588,6 +609,7 @@ __global__ void __launch_bounds__(pa_threads(N), 1) paged_attention_tc_kernel(
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (start->gap) paged_clear_gaps(rg, total, (size_t)H * R * 2, reinterpret_cast<uint8_t*>(out));
   const uint32_t tmem = warp_uniform(*tmem_slot);
   const int count = warp_uniform(start->count), b_0 = warp_uniform(start->b), rt_0 = warp_uniform(start->rt),
             tile_0 = warp_uniform(start->tile);

@@ -76,7 +76,8 @@ def paged_latent_attention(q: torch.Tensor, pages: torch.Tensor, block_table: to
     ``q [T, H, R + dr]`` holds each head's query multiplied by ``W_k`` (R)
     followed by its rotated part (dr).  Row ``t`` sees the cached rows up to its
     own position; the result ``[T, H, R]`` is the weighted sum of their latents.
-    A token that sees no row (its position is negative) gets zeros.  Rows at and
+    A token that sees no row (its position is negative) or that no sequence holds
+    (reported) gets zeros.  Rows at and
     past ``seq_lens`` may hold anything; those before it have to be finite, also
     for earlier tokens that do not see them (their weight there is zero, and zero
     times infinity is not).  ``q`` is copied if it is not contiguous.

@@ -42,3 +42,30 @@ def test_rotation_skips_positions_outside_its_tables(reported):
                      ("one position per token", (x, 24, 8, cos, sin, pos.long(), 1, 0, False))]:
         with pytest.raises(RuntimeError, match=match):
             C.rope_inplace(*a)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,rank", [(4, 64), (16, 512), (12, 192)])
+@pytest.mark.parametrize("cu", [[2, 5, 8], [0, 3, 7], [3, 6, 10], [0, 12, 10], [4, 2, 10]], ids=str)
+def test_attention_gives_zeros_to_tokens_of_no_sequence(cu, heads, rank, reported):
+    """Offsets that leave tokens out: those rows are zeros, the tokens of intact sequences get their result."""
+    from ops.paged import paged_latent_attention
+    g = torch.Generator(device="cuda").manual_seed(rank)
+    width, total = rank + 16, 10
+    pages = torch.randn(6, 64, width, device="cuda", generator=g).bfloat16()
+    table = _i32([[0, 1, 2], [3, 4, 5]], "cuda")
+    q = torch.randn(total, heads, width, device="cuda", generator=g).bfloat16()
+    lens = _i32([150, 90], "cuda")
+    del_me = torch.full((total, heads, rank), float("nan"), device="cuda", dtype=torch.bfloat16)
+    del del_me                                               # the result is likely to get this memory
+    out = paged_latent_attention(q, pages, table, _i32(cu, "cuda"), lens, rank, 0.1)
+    reported()
+    held = torch.zeros(total, dtype=torch.bool)
+    for b in range(2):
+        lo, hi = cu[b], cu[b + 1]
+        if lo < hi <= total:
+            held[lo:hi] = True
+            want = paged_latent_attention(q[lo:hi].contiguous(), pages, table[b:b + 1], _i32([0, hi - lo], "cuda"),
+                                          lens[b:b + 1], rank, 0.1)
+            torch.testing.assert_close(out[lo:hi].float(), want.float(), rtol=2.0 ** -6, atol=1e-3)
+    assert (out[~held.cuda()] == 0).all()
