@@ -324,7 +324,7 @@ class InferenceEngine:
                 self._moe(layer.ffn, xn, x)
             else:
                 self._dense_ffn(layer.ffn.w1.weight, layer.ffn.w3.weight, layer.ffn.w2.weight, xn, x)
-        x = x[(cu_seqlens[1:].long() - 1).clamp(min=0)]
+        x = x[(cu_seqlens[1:].long() - 1).clamp(0, T - 1)]
         logits = torch.empty(x.shape[0], self.Vp, dtype=BF16, device=self.device)
         C.linear_fwd(self._norm(x, m.norm.weight), self.bf16(m.head.weight), logits[:, :self.V])
         return logits[:, :self.V]

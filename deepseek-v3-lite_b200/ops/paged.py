@@ -34,13 +34,29 @@ from . import norm as norm_ops
 from ._ext import native
 
 
-def token_positions(cu_seqlens: torch.Tensor, seq_lens: torch.Tensor, total: int):
-    """``(sequence, position)`` of each of ``total`` new tokens (int64)."""
+def ragged_positions(cu_seqlens: torch.Tensor, seq_lens: torch.Tensor, total: int):
+    """``(sequence, position)`` of each of ``total`` new tokens (int64), without a look at the values on the host.
+
+    A token that no sequence holds gets a sequence in range and position -1,
+    which the kernels skip and report.
+    """
+    if total and not seq_lens.numel():
+        raise IndexError(f"{total} tokens without a sequence")
     t = torch.arange(total, device=cu_seqlens.device)
-    seq = torch.searchsorted(cu_seqlens[1:].long().contiguous(), t, right=True)
-    if total and not seq.is_cuda and int(seq[-1]) >= seq_lens.numel():
-        raise IndexError(f"cu_seqlens covers {int(cu_seqlens[-1])} of {total} tokens")
-    return seq, seq_lens.long()[seq] - cu_seqlens.long()[seq + 1] + t
+    cu, lens = cu_seqlens.long(), seq_lens.long()
+    seq = torch.searchsorted(cu[1:].contiguous(), t, right=True)
+    held = seq < lens.numel()
+    seq = seq.clamp(max=max(lens.numel() - 1, 0))
+    held &= t >= cu[seq]
+    return seq, torch.where(held, lens[seq] - cu[seq + 1] + t, -1)
+
+
+def token_positions(cu_seqlens: torch.Tensor, seq_lens: torch.Tensor, total: int):
+    """``ragged_positions``; on the CPU a token that no sequence holds raises ``IndexError``."""
+    seq, pos = ragged_positions(cu_seqlens, seq_lens, total)
+    if total and not pos.is_cuda and (int(cu_seqlens[0]) > 0 or int(cu_seqlens[-1]) < total):
+        raise IndexError(f"cu_seqlens covers {int(cu_seqlens[0])} to {int(cu_seqlens[-1])} of {total} tokens")
+    return seq, pos
 
 
 def latent_cache_append(pages: torch.Tensor, kv_a: torch.Tensor, weight: torch.Tensor, cos: torch.Tensor,

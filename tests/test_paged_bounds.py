@@ -69,3 +69,65 @@ def test_attention_gives_zeros_to_tokens_of_no_sequence(cu, heads, rank, reporte
                                           lens[b:b + 1], rank, 0.1)
             torch.testing.assert_close(out[lo:hi].float(), want.float(), rtol=2.0 ** -6, atol=1e-3)
     assert (out[~held.cuda()] == 0).all()
+
+
+def test_positions_of_tokens_that_no_sequence_holds():
+    """Before the first offset, past the last one, and without any sequence: no index leaves its range."""
+    from ops.paged import ragged_positions, token_positions
+    lens = _i32([10, 4])
+    for cu, want in [([0, 3, 5], [7, 8, 9, 2, 3]), ([1, 3, 5], [-1, 8, 9, 2, 3]), ([0, 3, 4], [7, 8, 9, 3, -1]),
+                     ([0, 0, 2], [2, 3, -1, -1, -1]), ([0, 9, 9], [1, 2, 3, 4, 5])]:
+        seq, pos = ragged_positions(_i32(cu), lens, 5)
+        assert pos.tolist() == want
+        assert seq.min() >= 0 and seq.max() < 2
+        if -1 in want:
+            with pytest.raises(IndexError, match="tokens"):
+                token_positions(_i32(cu), lens, 5)
+        else:
+            assert token_positions(_i32(cu), lens, 5)[1].tolist() == want
+    with pytest.raises(IndexError, match="without a sequence"):
+        ragged_positions(_i32([0]), _i32([]), 2)
+    assert ragged_positions(_i32([0]), _i32([]), 0)[1].numel() == 0
+
+
+STEP_CFG = {
+    "vocab_size": 1000, "dim": 256, "n_layers": 2, "n_heads": 4, "n_dense_layers": 1,
+    "n_routed_experts": 8, "n_shared_experts": 1, "n_activated_experts": 2, "inter_dim": 512,
+    "moe_inter_dim": 128, "kv_lora_rank": 64, "q_lora_rank": 0, "qk_nope_head_dim": 48,
+    "qk_rope_head_dim": 16, "v_head_dim": 64, "max_seq_len": 96, "rope_theta": 10000,
+    "rope_factor": 1.0, "mscale": 1.0, "mtp_depth": 1, "mtp_loss_weight": 0.3,
+    "attn_impl": "sdpa", "weight_tying": True,
+}
+
+
+@pytest.mark.gpu
+def test_model_step_survives_bad_metadata(reported):
+    """Offsets that leave tokens out or pass them, positions past the model's length, unknown token ids: reported,
+    and the sequences that are in order get their logits."""
+    from models.transformer import Transformer
+    from ops.paged import PagedLatentCache, paged_step
+    torch.manual_seed(0)
+    model = Transformer(STEP_CFG).cuda().eval()
+    g = torch.Generator(device="cuda").manual_seed(2)
+    tokens = torch.randint(0, 1000, (12,), device="cuda", generator=g)
+    table = torch.arange(24, dtype=torch.int32, device="cuda").view(2, 12)
+
+    def step(cu, lens, toks=tokens):
+        cache = PagedLatentCache(STEP_CFG, 24, 16, "cuda")
+        cache.pages.zero_()
+        return paged_step(model, toks, cache, table, _i32(cu, "cuda"), _i32(lens, "cuda")).float()
+
+    want = step([0, 5, 12], [5, 7])
+    for cu, lens in [([0, 5, 9], [5, 4]), ([0, 5, 20], [5, 15]), ([0, 5, 12], [5, 120]), ([0, 5, 12], [5, 3]),
+                     ([0, 5, 12], [5, -9]), ([0, 5, 12], [5, 1 << 30])]:
+        got = step(cu, lens)
+        reported()
+        torch.testing.assert_close(got[0], want[0], rtol=2e-2, atol=2e-2)
+    got = step([3, 5, 12], [2, 7])
+    reported()
+    torch.testing.assert_close(got[1], want[1], rtol=2e-2, atol=2e-2)
+    wrong = tokens.clone()
+    wrong[6], wrong[7] = 1000, -1
+    got = step([0, 5, 12], [5, 7], wrong)
+    reported()
+    torch.testing.assert_close(got[0], want[0], rtol=2e-2, atol=2e-2)
