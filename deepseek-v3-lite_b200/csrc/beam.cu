@@ -354,7 +354,9 @@ __global__ void __launch_bounds__(kCopyThreads) beam_reorder_kernel(uint4* __res
   const int b = blockIdx.z, layer = blockIdx.y;
   const bool writes_table = (int)blockIdx.x == parts * splits;
   if (writes_table && layer > 0) return;
-  const int len = lens[b];
+  // a length outside the table is reported; a negative one counts as zero
+  const int given = lens[b], len = max(given, 0);
+  if (writes_table && threadIdx.x == 0 && (given < 0 || given > (long)cols * page)) record_error(status, DSV3_ERR_BOUNDS);
   const int col = len / page, rem = len % page;
   const int part = blockIdx.x % parts, split = blockIdx.x / parts;
   const int n16 = rem * row16;

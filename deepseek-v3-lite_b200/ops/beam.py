@@ -67,6 +67,9 @@ def beam_reorder(pages: torch.Tensor, block_table: torch.Tensor, parents: torch.
     layer (in place).  Later columns, and the current one when it is empty,
     stay each beam's own, so the pages being written are always distinct
     within an entry if they were to begin with.
+
+    On CUDA a parent, page or length out of range is skipped and reported by
+    ``ops._ext.check_status`` (a negative length counts as zero).
     """
     if pages.is_cuda:
         return native().beam_reorder(pages, block_table, parents, seq_lens)

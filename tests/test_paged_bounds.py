@@ -131,3 +131,16 @@ def test_model_step_survives_bad_metadata(reported):
     got = step([0, 5, 12], [5, 7], wrong)
     reported()
     torch.testing.assert_close(got[0], want[0], rtol=2e-2, atol=2e-2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("length", [-1, -16, -17, -100000, -(1 << 31), 49, 64, 100000, (1 << 31) - 1])
+def test_reorder_reports_lengths_outside_the_table(length, reported):
+    from ops.beam import beam_reorder
+    pages = torch.randn(2, 12, 16, 32, device="cuda").bfloat16()
+    before = pages.clone()
+    table = torch.arange(12, dtype=torch.int32, device="cuda").view(4, 3)
+    out = beam_reorder(pages, table, _i32([[1, 1, 2, 1]], "cuda"), _i32([length], "cuda"))
+    reported()
+    assert torch.equal(pages, before)
+    assert torch.equal(out, table if length < 0 else table[[1, 1, 2, 1]])
