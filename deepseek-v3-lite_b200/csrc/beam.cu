@@ -432,8 +432,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> beam_select(const at:
                   (logits.scalar_type() == at::kFloat || logits.scalar_type() == at::kBFloat16),
               op, ": logits must be a CUDA bf16 or fp32 tensor [B, K, V] with unit stride in the last dimension");
   const int64_t B = logits.size(0), K = logits.size(1), V = logits.size(2);
-  TORCH_CHECK(K >= 1 && K <= kMaxBeams && V >= K && K * V < (1ll << 31), op,
-              ": 1 to 32 beams, at least as many tokens as beams and K * V below 2^31");
+  // (the last segment of a row counts up to 4,095 past V in 32 bits)
+  TORCH_CHECK(K >= 1 && K <= kMaxBeams && V >= K && K * V < (1ll << 31) - 4096, op,
+              ": 1 to 32 beams, at least as many tokens as beams and K * V below 2^31 - 4096");
   TORCH_CHECK(scores.scalar_type() == at::kFloat && scores.is_contiguous() && scores.dim() == 2 &&
                   scores.size(0) == B && scores.size(1) == K && scores.device() == logits.device(),
               op, ": scores must be a contiguous fp32 tensor [B, K]");

@@ -144,3 +144,13 @@ def test_reorder_reports_lengths_outside_the_table(length, reported):
     reported()
     assert torch.equal(pages, before)
     assert torch.equal(out, table if length < 0 else table[[1, 1, 2, 1]])
+
+
+@pytest.mark.gpu
+def test_select_refuses_vocabularies_whose_segments_pass_32_bits():
+    from ops.beam import beam_select
+    scores = torch.zeros(0, 1, device="cuda")
+    for vocab in ((1 << 31) - 100, (1 << 31) - 4096):
+        with pytest.raises(RuntimeError, match="2\\^31"):
+            beam_select(torch.empty(0, 1, vocab, device="cuda"), scores)
+    assert beam_select(torch.empty(0, 1, (1 << 31) - 4097, device="cuda"), scores)[0].shape == (0, 1)
