@@ -487,8 +487,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> beam_select(const at:
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   C10_CUDA_CHECK(launch_dependent(beam_pick_kernel, dim3((unsigned)B), kPickThreads, st, (const float2*)stat,
                                   (const uint64_t*)cand, (const float*)scores.data_ptr<float>(), done, (int)K, (int)V,
-                                  nseg, chunk, runs, (int)eos, o_score.data_ptr<float>(), o_parent.data_ptr<int>(),
-                                  o_token.data_ptr<int>(), o_done.data_ptr<bool>()));
+                                  nseg, chunk, runs, eos >= 0 && eos < V ? (int)eos : -1, o_score.data_ptr<float>(),
+                                  o_parent.data_ptr<int>(), o_token.data_ptr<int>(), o_done.data_ptr<bool>()));
   return {o_score, o_parent, o_token, o_done};
 }
 
