@@ -34,7 +34,7 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 __device__ __forceinline__ uint64_t entry_of(uint32_t key, uint32_t index) { return (uint64_t)key << 32 | ~index; }
 __device__ __forceinline__ uint32_t entry_index(uint64_t e) { return ~(uint32_t)e; }
 
-// A logit as the selection sees it: NaN counts as -inf, +inf (below) as the largest
+// A logit or score as the selection sees it: NaN counts as -inf, +inf (below) as the largest
 // finite float, so that the log-sum-exp of a row is always defined; -0 becomes 0,
 // whose key differs.
 constexpr float kLargest = 3.402823466e38f;
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const float2* _
     if (lane == 0) {
       s_max[r] = m;
       s_log[r] = logf(s);
-      s_score[r] = scores[row0 + r] + 0.f;          // (-0 becomes 0)
+      s_score[r] = fminf(number_of(scores[row0 + r]), kLargest);
       s_done[r] = done;
       s_runs[r] = n;
     }

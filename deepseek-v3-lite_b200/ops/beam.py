@@ -23,8 +23,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: Optional[t
     Candidates are ordered by score (of one beam: by logit), ties by ``(k, v)``.
 
     Returns ``(scores [B, K] fp32, parents [B, K] int32, tokens [B, K] int32,
-    finished [B, K] bool)``, best first.  A NaN logit counts as ``-inf`` and an
-    infinite one as the largest finite float; a row of ``-inf`` offers nothing
+    finished [B, K] bool)``, best first.  A NaN logit or score counts as ``-inf`` and
+    an infinite one as the largest finite float; a row of ``-inf`` offers nothing
     (score ``-inf``).  Up to 32 beams on CUDA.
     """
     if logits.is_cuda:
@@ -38,6 +38,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: Optional[t
     ninf = torch.tensor(float("-inf"))
     x = torch.where(torch.isnan(logits), ninf.to(logits.dtype), logits).float().clamp(max=big)
     top = x.amax(-1, keepdim=True).clamp(min=-big)
+    scores = torch.where(torch.isnan(scores), ninf, scores).clamp(max=big)
     total = torch.exp(x - top).sum(-1, keepdim=True)
     logp = torch.where(total > 0, (x - top) - torch.log(total), ninf)
     if finished is not None:
