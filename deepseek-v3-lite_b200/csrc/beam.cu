@@ -38,8 +38,19 @@ __device__ __forceinline__ uint32_t entry_index(uint64_t e) { return ~(uint32_t)
 // finite float, so that the log-sum-exp of a row is always defined; -0 becomes 0,
 // whose key differs.
 constexpr float kLargest = 3.402823466e38f;
+constexpr uint32_t kLowestKey = 0x007fffffu;   // of -inf
 __device__ __forceinline__ float number_of(float x) { return fmaxf(x, -INFINITY) + 0.f; }
 __device__ __forceinline__ float number_of(bf16 x) { return number_of(__bfloat162float(x)); }
+
+// Logits that differ by more than kTieWindow have different scores where
+// 3 (max - logit) + |score| < kTieReach: a score is score + ((x - max) - log sum),
+// three roundings of at most 2^-24 of their results, and log sum is at most 22 (V <
+// 2^31), so that two scores differ by 2^-23 (3 (max - x) + 44 + |score|) less than
+// their logits, at most.  Half of the window is kept for its own rounding.
+constexpr float kTieWindow = 1.f / 2048, kTieReach = 2000.f;
+__device__ __forceinline__ uint32_t below_window(uint32_t key) {
+  return key <= kLowestKey ? key : order_key(key_value(key) - kTieWindow);
+}
 
 // e^x for x <= 0, flushed to zero where it would be denormal.
 __device__ __forceinline__ float exp_of(float x) { return ex2_approx(x * 1.4426950408889634f); }
@@ -127,7 +138,8 @@ __device__ __forceinline__ void cta_rank(int k, uint32_t threshold, bool any, in
 
 // A CTA walks `chunk` consecutive segments of PER * THREADS logits, rows one after
 // another, and leaves one record per row that it touches: maximum, sum of
-// exponentials and the K largest of its part.  Every thread keeps a running
+// exponentials, the K largest of its part and, of the logits left out, the largest
+// that lies within kTieWindow of them.  Every thread keeps a running
 // maximum and sum, the CTA a list of the K best so far; a segment that holds
 // nothing above the last of them costs one barrier.  The logits of the next
 // segment are on their way while this one is looked at.  A thread's elements go
@@ -139,10 +151,11 @@ __global__ void __launch_bounds__(THREADS, 3) beam_scan_kernel(const T* __restri
                                                                             int K, int V,
                                                                             const bool* __restrict__ finished,
                                                                             float2* __restrict__ stat,
-                                                                            uint64_t* __restrict__ cand) {
+                                                                            uint64_t* __restrict__ cand,
+                                                                            uint32_t* __restrict__ left) {
   constexpr int VE = 16 / sizeof(T), NV = PER / VE, W = THREADS / 32;
   __shared__ float2 red[W];
-  __shared__ uint64_t best[2][kMaxBeams];
+  __shared__ uint64_t best[2][kMaxBeams + 1];
   __shared__ int s_n;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -184,7 +197,7 @@ __global__ void __launch_bounds__(THREADS, 3) beam_scan_kernel(const T* __restri
   };
   bool next_live = u0 < u1 && fetch();
   float m = -kLargest, s = 0.f;
-  uint32_t last = 0;                      // key of the K-th best so far
+  uint32_t floor = 1;                     // key that later logits have to reach
   int cur = 0;
   for (int u = u0; u < u1; ++u) {
     const bool live = next_live, begin = u == u0 || seg == 0, end = u + 1 == u1 || seg == nseg - 1;
@@ -223,11 +236,11 @@ __global__ void __launch_bounds__(THREADS, 3) beam_scan_kernel(const T* __restri
     m = now;
     const uint32_t key = first < V ? order_key(top) : 0u;
     if (tid == 0) s_n = 0;
-    const uint32_t threshold = begin ? cta_threshold<THREADS>(K, key) : last + 1;   // later indices lose ties
+    const uint32_t threshold = begin ? below_window(cta_threshold<THREADS>(K, key)) : floor;
     const bool any = key >= threshold && key > 0;
     if (begin || __syncthreads_or(any)) {
       cta_rank<THREADS>(
-          K, threshold, any || (!begin && tid < K), &s_n,
+          K + 1, threshold, any || (!begin && tid <= K), &s_n,
           [&](uint32_t least, auto&& f) {
             const float low = key_value(least);          // (a NaN for keys below that of -inf)
 #pragma unroll
@@ -237,12 +250,16 @@ __global__ void __launch_bounds__(THREADS, 3) beam_scan_kernel(const T* __restri
                 const uint32_t k = order_key(v[i]);
                 if (at < V && k >= least) f(entry_of(k, (uint32_t)at));
               }
-            if (!begin && tid < K && best[cur][tid] != 0) f(best[cur][tid]);
+            if (!begin && tid <= K && best[cur][tid] != 0) f(best[cur][tid]);
           },
           [&](int rank, uint64_t e) { best[cur ^ 1][rank] = e; });
       __syncthreads();
       cur ^= 1;
-      last = (uint32_t)(best[cur][K - 1] >> 32);
+      // Later indices lose ties of equal logits, but logits in the window below the
+      // K-th best are ranked too, so that the one after it is known; where that one
+      // equals it already (masked rows) nothing is left to know.
+      const uint32_t last = (uint32_t)(best[cur][K - 1] >> 32), next = (uint32_t)(best[cur][K] >> 32);
+      floor = last == next ? last + 1 : below_window(last);
     }
     if (end) {
       const float wm = warp_max(m);
@@ -251,6 +268,7 @@ __global__ void __launch_bounds__(THREADS, 3) beam_scan_kernel(const T* __restri
       __syncthreads();
       const size_t at = (size_t)this_row * runs + (blockIdx.x - this_row * nseg / chunk);
       if (tid < K) cand[at * K + tid] = best[cur][tid];
+      if (tid == K) left[at] = (uint32_t)(best[cur][K] >> 32);
       if (warp == W - 1) {
         const float2 r = lane < W ? red[lane] : make_float2(-kLargest, 0.f);
         const float M = warp_max(r.x);
@@ -261,9 +279,28 @@ __global__ void __launch_bounds__(THREADS, 3) beam_scan_kernel(const T* __restri
   }
 }
 
+// The logits again, for the rare case below.
+struct BeamLogits {
+  const void* at;
+  long ldb, ldk;
+  bool narrow;                // bf16
+  __device__ __forceinline__ float operator()(int b, int r, int v) const {
+    const long i = b * ldb + r * ldk + v;
+    const float x = narrow ? number_of(static_cast<const bf16*>(at)[i]) : number_of(static_cast<const float*>(at)[i]);
+    return fminf(x, kLargest);
+  }
+};
+
 // One CTA per batch entry: log-sum-exp of its beams, then the K best candidates.
-__global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const float2* __restrict__ stat,
+//
+// A row's part keeps its K largest logits, and a score is a rounded and so not
+// strictly growing function of the logit: a candidate that a part left out cannot
+// beat the K-th best score, but it can equal it at a lower index.  Where the parts'
+// records do not rule that out, and only there, the entry's rows are read again for
+// the candidates that score exactly the K-th best.
+__global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(BeamLogits logits, const float2* __restrict__ stat,
                                                                  const uint64_t* __restrict__ cand,
+                                                                 const uint32_t* __restrict__ left,
                                                                  const float* __restrict__ scores,
                                                                  const bool* __restrict__ finished, int K, int V,
                                                                  int nseg, int chunk, int runs, int eos,
@@ -274,6 +311,8 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const float2* _
   __shared__ float s_max[kMaxBeams], s_log[kMaxBeams], s_score[kMaxBeams];
   __shared__ bool s_done[kMaxBeams];
   __shared__ int s_runs[kMaxBeams], s_n;
+  __shared__ float s_val[kMaxBeams];      // the scores chosen
+  __shared__ int s_ties[kPickThreads / 32];
   const size_t row0 = (size_t)b * K;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   for (int r = warp; r < K; r += kPickThreads / 32) {
@@ -298,6 +337,15 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const float2* _
   if (tid == 0) s_n = 0;
   __syncthreads();
   const int per = runs * K;               // candidates per beam, at most
+  // score of a logit, and whether a beam has such candidates (the others: -inf)
+  auto score_of = [&](int r, float x) { return s_score[r] + ((x - s_max[r]) - s_log[r]); };
+  auto live = [&](int r) { return !s_done[r] && s_score[r] > -INFINITY && s_log[r] > -INFINITY; };
+  // smallest logit that part c % runs of beam c / runs kept, 0 if it kept all
+  auto least_kept = [&](int c) -> uint32_t {
+    const int r = c / runs;
+    return c < K * runs && live(r) && c % runs < s_runs[r] ? cand[row0 * per + (size_t)c * K + K - 1] >> 32 : 0;
+  };
+  const uint32_t least0 = least_kept(tid);       // (on its way while the candidates are ranked)
   auto candidate = [&](int c) -> uint64_t {
     const int r = c / per, i = c % per;
     const float sc = s_score[r];
@@ -307,7 +355,7 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const float2* _
       if (i >= K) return 0;
       v = i == 0 ? eos : (i - 1 < eos ? i - 1 : i);
       if (i == 0) val = sc;
-    } else if (!(sc > -INFINITY) || s_log[r] == -INFINITY) {
+    } else if (!live(r)) {
       if (i >= K) return 0;
       v = i;
     } else {
@@ -315,9 +363,15 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const float2* _
       const uint64_t e = cand[row0 * per + c];
       if (e == 0) return 0;
       v = entry_index(e);
-      val = sc + ((key_value((uint32_t)(e >> 32)) - s_max[r]) - s_log[r]);
+      val = score_of(r, key_value((uint32_t)(e >> 32)));
     }
     return v < (uint32_t)V ? entry_of(order_key(val), r * V + v) : 0;
+  };
+  auto choose = [&](int rank, float val, int r, int v) {
+    o_score[row0 + rank] = val;
+    o_parent[row0 + rank] = r;
+    o_token[row0 + rank] = v;
+    o_done[row0 + rank] = s_done[r] || v == eos;
   };
   uint32_t top = 0;
   for (int c = tid; c < K * per; c += kPickThreads) top = max(top, (uint32_t)(candidate(c) >> 32));
@@ -332,12 +386,79 @@ __global__ void __launch_bounds__(kPickThreads) beam_pick_kernel(const float2* _
       },
       [&](int rank, uint64_t e) {
         const uint32_t at = entry_index(e);
-        const int p = at / V, v = at % V;
-        o_score[row0 + rank] = key_value((uint32_t)(e >> 32));
-        o_parent[row0 + rank] = p;
-        o_token[row0 + rank] = v;
-        o_done[row0 + rank] = s_done[p] || v == eos;
+        s_val[rank] = key_value((uint32_t)(e >> 32));
+        choose(rank, s_val[rank], at / V, at % V);
       });
+  __syncthreads();
+  const float cut = s_val[K - 1];
+  bool tie = false;
+  for (int c = tid; c < K * runs; c += kPickThreads) {
+    const int r = c / runs;
+    const uint32_t least = c == tid ? least0 : least_kept(c);
+    const float x = key_value(least);
+    if (least == 0 || score_of(r, x) != cut) continue;
+    if (x > -INFINITY && !(3.f * (s_max[r] - x) + fabsf(s_score[r]) < kTieReach)) {
+      tie = true;
+      continue;
+    }
+    const uint32_t out = left[row0 * runs + c];
+    if (out == least) {
+      // equal logits at higher indices are left out, which does no harm unless a
+      // smaller logit may score the same, or a larger one, perhaps behind them, does
+      const uint32_t step = logits.narrow ? 0x10000u : 1u;     // to the next value of the logits' type
+      const uint64_t* list = cand + row0 * per + (size_t)c * K;
+      int j = K - 2;
+      while (j >= 0 && (uint32_t)(list[j] >> 32) == least) --j;
+      tie |= (x > -INFINITY && score_of(r, key_value(least - step)) == cut) ||
+             (j >= 0 && score_of(r, key_value((uint32_t)(list[j] >> 32))) == cut);
+    } else if (out != 0) {
+      tie |= score_of(r, key_value(out)) == cut;
+    }
+  }
+  if (!__syncthreads_or(tie)) return;
+  // the scores above the cut stand; behind them, the lowest indices that score it
+  int n = 0;
+  while (s_val[n] > cut) ++n;
+  constexpr int PER = 8;                  // consecutive tokens of a thread
+  for (int r = 0; r < K && n < K; ++r) {
+    const bool alive = live(r);
+    if (alive && score_of(r, s_max[r]) < cut) continue;
+    if (!alive && cut > -INFINITY) {      // at most the end token of a finished beam
+      if (s_done[r] && s_score[r] == cut) {
+        if (tid == 0) choose(n, cut, r, eos);
+        ++n;
+      }
+      continue;
+    }
+    for (int v0 = 0; v0 < V && n < K; v0 += PER * kPickThreads) {
+      const int first = v0 + tid * PER;
+      unsigned hit = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int v = first + i;
+        if (v < V) {
+          const float val = alive ? score_of(r, logits(b, r, v)) : s_done[r] && v == eos ? s_score[r] : -INFINITY;
+          hit |= (unsigned)(val == cut) << i;
+        }
+      }
+      if (!__syncthreads_or(hit)) continue;
+      int upto = __popc(hit);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+      }
+      if (lane == 31) s_ties[warp] = upto;
+      __syncthreads();
+      int rank = n + upto - __popc(hit);
+      for (int w = 0; w < kPickThreads / 32; ++w) {
+        if (w < warp) rank += s_ties[w];
+        n += s_ties[w];
+      }
+      for (; hit != 0 && rank < K; hit &= hit - 1) choose(rank++, cut, r, first + __ffs(hit) - 1);
+      __syncthreads();                    // the counts are read
+    }
+  }
 }
 
 // Grid (x, layer, group).  CTA x < parts * splits copies 16 KB of the page that
@@ -357,7 +478,8 @@ __global__ void __launch_bounds__(kCopyThreads) beam_reorder_kernel(uint4* __res
   if (writes_table && layer > 0) return;
   // a length outside the table is reported; a negative one counts as zero
   const int given = lens[b], len = max(given, 0);
-  if (writes_table && threadIdx.x == 0 && (given < 0 || given > (long)cols * page)) record_error(status, DSV3_ERR_BOUNDS);
+  if (writes_table && threadIdx.x == 0 && (given < 0 || given > (long)cols * page))
+    record_error(status, DSV3_ERR_BOUNDS);
   const int col = len / page, rem = len % page;
   const int part = blockIdx.x % parts, split = blockIdx.x / parts;
   const int n16 = rem * row16;
@@ -467,13 +589,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> beam_select(const at:
                        logits.stride(1) * es % 16 == 0;
   const int64_t units = B * K * nseg, ctas = sms * 3;
   const int chunk = (int)((units + ctas - 1) / ctas), runs = (nseg - 1) / chunk + 2;   // parts of a row, at most
-  auto work = make({B * K * runs * (1 + K) * 2}, at::kFloat);
+  auto work = make({B * K * runs * (3 + 2 * K)}, at::kFloat);
   float2* stat = reinterpret_cast<float2*>(work.data_ptr());
   uint64_t* cand = reinterpret_cast<uint64_t*>(stat + B * K * runs);
+  uint32_t* left = reinterpret_cast<uint32_t*>(cand + B * K * runs * K);
 #define DSV3_SCAN(T_, PER_, ALIGNED_)                                                                          \
   beam_scan_kernel<T_, 256, PER_, ALIGNED_><<<(unsigned)((units + chunk - 1) / chunk), 256, 0, st>>>(          \
       reinterpret_cast<const T_*>(logits.data_ptr()), logits.stride(0), logits.stride(1), (int)units, nseg, chunk, \
-      runs, (int)K, (int)V, done, stat, cand)
+      runs, (int)K, (int)V, done, stat, cand, left)
 #define DSV3_SCAN_TYPE(T_)                              \
   do {                                                  \
     if (span == 4096 && aligned) DSV3_SCAN(T_, 16, true); \
@@ -486,9 +609,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> beam_select(const at:
 #undef DSV3_SCAN_TYPE
 #undef DSV3_SCAN
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  C10_CUDA_CHECK(launch_dependent(beam_pick_kernel, dim3((unsigned)B), kPickThreads, st, (const float2*)stat,
-                                  (const uint64_t*)cand, (const float*)scores.data_ptr<float>(), done, (int)K, (int)V,
-                                  nseg, chunk, runs, eos >= 0 && eos < V ? (int)eos : -1, o_score.data_ptr<float>(),
+  const BeamLogits again{logits.data_ptr(), (long)logits.stride(0), (long)logits.stride(1),
+                         logits.scalar_type() == at::kBFloat16};
+  C10_CUDA_CHECK(launch_dependent(beam_pick_kernel, dim3((unsigned)B), kPickThreads, st, again, (const float2*)stat,
+                                  (const uint64_t*)cand, (const uint32_t*)left,
+                                  (const float*)scores.data_ptr<float>(), done, (int)K, (int)V, nseg, chunk, runs,
+                                  eos >= 0 && eos < V ? (int)eos : -1, o_score.data_ptr<float>(),
                                   o_parent.data_ptr<int>(), o_token.data_ptr<int>(), o_done.data_ptr<bool>()));
   return {o_score, o_parent, o_token, o_done};
 }

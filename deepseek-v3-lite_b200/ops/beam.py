@@ -20,7 +20,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: Optional[t
     of each beam so far; ``-inf`` for a beam that holds nothing yet).  Candidate
     ``(k, v)`` scores ``scores[k] + log_softmax(logits[k])[v]``; a beam with
     ``finished[b, k]`` offers only ``eos_token_id``, at its unchanged score.
-    Candidates are ordered by score (of one beam: by logit), ties by ``(k, v)``.
+    Candidates are ordered by their fp32 score, ties by ``(k, v)``.
 
     Returns ``(scores [B, K] fp32, parents [B, K] int32, tokens [B, K] int32,
     finished [B, K] bool)``, best first.  A NaN logit or score counts as ``-inf`` and
