@@ -158,6 +158,9 @@ def paged_step(model, tokens: torch.Tensor, cache: PagedLatentCache, block_table
     each sequence, ``[B, vocab]`` (a sequence without new tokens gets an
     unspecified row).  Metadata as above.
     """
+    if not tokens.numel():                   # every slot idle
+        return model.head.weight.new_zeros(seq_lens.numel(), model.config["vocab_size"],
+                                           dtype=torch.bfloat16 if tokens.is_cuda else None)
     if tokens.is_cuda:
         return model.native_inference().forward_paged(tokens, cache, block_table, cu_seqlens, seq_lens)
     from .decode import _row_rope

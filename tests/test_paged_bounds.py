@@ -154,3 +154,32 @@ def test_select_refuses_vocabularies_whose_segments_pass_32_bits():
         with pytest.raises(RuntimeError, match="2\\^31"):
             beam_select(torch.empty(0, 1, vocab, device="cuda"), scores)
     assert beam_select(torch.empty(0, 1, (1 << 31) - 4097, device="cuda"), scores)[0].shape == (0, 1)
+
+
+def _empty_step(cfg, device):
+    from models.transformer import Transformer
+    from ops.paged import PagedLatentCache, paged_step
+    torch.manual_seed(0)
+    model = Transformer(cfg).to(device).eval()
+    dtype = torch.bfloat16 if device == "cuda" else torch.float32
+    cache = PagedLatentCache(cfg, 6, 8, device, dtype)
+    cache.pages.normal_()
+    before = cache.pages.clone()
+    for batch in (3, 0):
+        out = paged_step(model, torch.zeros(0, dtype=torch.long, device=device), cache,
+                         torch.zeros(batch, 2, dtype=torch.int32, device=device), _i32([0] * (batch + 1), device),
+                         _i32([4] * batch, device))
+        assert out.shape == (batch, cfg["vocab_size"])
+    assert torch.equal(cache.pages, before)
+
+
+def test_step_without_new_tokens(small_cfg):
+    """Every slot of the batch idle: one row of logits per sequence, and the cache as it was."""
+    _empty_step(small_cfg, "cpu")
+
+
+@pytest.mark.gpu
+def test_step_without_new_tokens_on_the_kernels():
+    from ops._ext import check_status
+    _empty_step(STEP_CFG, "cuda")
+    check_status()
