@@ -10,6 +10,7 @@ from typing import Optional, Tuple
 import torch
 
 from ._ext import native
+from .paged import check_range
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: Optional[torch.Tensor] = None,
@@ -70,12 +71,19 @@ def beam_reorder(pages: torch.Tensor, block_table: torch.Tensor, parents: torch.
     within an entry if they were to begin with.
 
     On CUDA a parent, page or length out of range is skipped and reported by
-    ``ops._ext.check_status`` (a negative length counts as zero).
+    ``ops._ext.check_status`` (a negative length counts as zero); on the CPU it
+    raises ``IndexError``.
     """
     if pages.is_cuda:
         return native().beam_reorder(pages, block_table, parents, seq_lens)
     bsz, beams = parents.shape
     page = pages.shape[2]
+    check_range("parent", parents, beams)
+    check_range("length", seq_lens, block_table.shape[1] * page + 1)
+    for b in range(bsz):                     # all checks before the first page is written
+        col, rem = divmod(int(seq_lens[b]), page)
+        if rem:
+            check_range("page", block_table[b * beams:(b + 1) * beams, col], pages.shape[1])
     out = block_table.clone()
     for b in range(bsz):
         col, rem = divmod(int(seq_lens[b]), page)

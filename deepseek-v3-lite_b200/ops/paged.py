@@ -34,6 +34,13 @@ from . import norm as norm_ops
 from ._ext import native
 
 
+def check_range(what: str, values: torch.Tensor, end: int) -> torch.Tensor:
+    """``values`` of a CPU form, all in ``[0, end)``; else ``IndexError`` (a negative one would count from the end)."""
+    if values.numel() and (int(values.min()) < 0 or int(values.max()) >= end):
+        raise IndexError(f"{what} {int(values.min())} to {int(values.max())}, not in 0 to {end - 1}")
+    return values
+
+
 def ragged_positions(cu_seqlens: torch.Tensor, seq_lens: torch.Tensor, total: int):
     """``(sequence, position)`` of each of ``total`` new tokens (int64), without a look at the values on the host.
 
@@ -74,13 +81,15 @@ def latent_cache_append(pages: torch.Tensor, kv_a: torch.Tensor, weight: torch.T
         return pages
     rank, page = weight.numel(), pages.shape[1]
     seq, pos = token_positions(cu_seqlens, seq_lens, kv_a.shape[0])
+    check_range("position", pos, min(cos.shape[0], block_table.shape[1] * page))
     x = kv_a.float()
     lat, pe = x[:, :rank], x[:, rank:]
     lat = lat * torch.rsqrt(lat.square().mean(-1, keepdim=True) + eps) * weight
     c, s = cos[pos], sin[pos]
     a, b = pe[:, 0::2], pe[:, 1::2]
     pe = torch.stack([a * c - b * s, a * s + b * c], dim=-1).flatten(1)
-    pages[block_table.long()[seq, pos // page], pos % page] = torch.cat([lat, pe], 1).to(pages.dtype)
+    ids = check_range("page", block_table.long()[seq, pos // page], pages.shape[0])
+    pages[ids, pos % page] = torch.cat([lat, pe], 1).to(pages.dtype)
     return pages
 
 
@@ -108,7 +117,7 @@ def paged_latent_attention(q: torch.Tensor, pages: torch.Tensor, block_table: to
         if hi <= lo or n <= 0:
             continue
         key = torch.arange(n)
-        kv = pages[block_table[b].long()[key // page], key % page].float()
+        kv = pages[check_range("page", block_table[b].long()[key // page], pages.shape[0]), key % page].float()
         pos = torch.arange(n - (hi - lo), n)
         s = torch.einsum("thd,jd->thj", q[lo:hi].float(), kv) * scale
         s = s.masked_fill((key[None, :] > pos[:, None])[:, None, :], float("-inf"))

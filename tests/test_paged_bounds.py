@@ -183,3 +183,40 @@ def test_step_without_new_tokens_on_the_kernels():
     from ops._ext import check_status
     _empty_step(STEP_CFG, "cuda")
     check_status()
+
+
+def test_cpu_forms_refuse_indices_below_zero():
+    """Python would count them from the end of the tensor: rows of other sequences."""
+    from ops.beam import beam_reorder
+    from ops.paged import latent_cache_append, paged_latent_attention
+    pages = torch.randn(4, 8, 24)
+    before = pages.clone()
+    table = _i32([[1, 0], [2, 3]])
+    w, cos = torch.ones(16), torch.ones(16, 4)
+
+    def append(rows, tab, cu, lens, **kw):
+        latent_cache_append(pages, torch.randn(rows, 24), w, kw.get("cos", cos), kw.get("cos", cos), tab, _i32(cu),
+                            _i32(lens))
+
+    with pytest.raises(IndexError, match="position"):
+        append(3, table, [0, 3, 3], [1, 5])                   # positions -2, -1, 0
+    with pytest.raises(IndexError, match="position"):
+        append(1, table, [0, 1, 1], [12, 5], cos=torch.ones(8, 4))
+    with pytest.raises(IndexError, match="page"):
+        append(1, _i32([[-1, 0], [2, 3]]), [0, 1, 1], [3, 5])
+    with pytest.raises(IndexError, match="page"):
+        append(1, _i32([[4, 0], [2, 3]]), [0, 1, 1], [3, 5])
+    with pytest.raises(IndexError):
+        append(1, table, [0, 1, 1], [17, 5], cos=torch.ones(32, 4))
+    with pytest.raises(IndexError, match="page"):
+        paged_latent_attention(torch.randn(1, 2, 24), pages, _i32([[-3, 0], [2, 3]]), _i32([0, 1, 1]), _i32([9, 5]), 16,
+                               0.2)
+    stack = pages[None].clone()
+    for match, par, tab, length in [("parent", [[0, -1]], table, 5), ("parent", [[0, 2]], table, 5),
+                                    ("length", [[0, 0]], table, -3), ("length", [[0, 0]], table, 17),
+                                    ("page", [[0, 0]], _i32([[-1, 0], [2, 3]]), 5),
+                                    ("page", [[0, 0]], _i32([[1, 0], [4, 3]]), 5)]:
+        with pytest.raises(IndexError, match=match):
+            beam_reorder(stack, tab, _i32(par), _i32([length]))
+    assert torch.equal(pages, before) and torch.equal(stack[0], before)
+    assert beam_reorder(stack, table, _i32([[0, 0]]), _i32([16])).tolist() == [[1, 0], [1, 0]]
