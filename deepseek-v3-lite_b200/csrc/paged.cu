@@ -59,7 +59,7 @@ __device__ __forceinline__ bf16* append_row(const Ragged& rg, int t, int lane, i
                                             long ld_row, int* pos, unsigned int* status) {
   const int b = ragged_seq(rg, t, lane);
   int pg = -1, col = 0;
-  if (b < rg.B) {
+  if (b < rg.B && t >= rg.cu[b]) {          // (not in front of the first offset)
     *pos = rg.lens[b] - rg.cu[b + 1] + t;
     col = *pos / rg.page;
     if (*pos >= 0 && *pos < npos && col < rg.cols) pg = rg.table[b * rg.ldt + col];

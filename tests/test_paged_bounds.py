@@ -220,3 +220,19 @@ def test_cpu_forms_refuse_indices_below_zero():
             beam_reorder(stack, tab, _i32(par), _i32([length]))
     assert torch.equal(pages, before) and torch.equal(stack[0], before)
     assert beam_reorder(stack, table, _i32([[0, 0]]), _i32([16])).tolist() == [[1, 0], [1, 0]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rank,rope", [(64, 16), (16, 12)], ids=["by_16_bytes", "by_elements"])
+def test_append_skips_tokens_of_no_sequence(rank, rope, reported):
+    """In front of the first offset and past the last one: nothing is written, the others are."""
+    from ops.paged import latent_cache_append
+    width = rank + rope
+    pages = torch.zeros(6, 16, 96, device="cuda", dtype=torch.bfloat16)[..., :width]
+    table = _i32([[0, 1, 2], [3, 4, 5]], "cuda")
+    x = torch.randn(9, width, device="cuda")
+    w, cos = torch.ones(rank, device="cuda"), torch.ones(48, rope // 2, device="cuda")
+    latent_cache_append(pages, x, w, cos, torch.zeros_like(cos), table, _i32([3, 5, 7], "cuda"), _i32([20, 33], "cuda"))
+    reported()
+    written = (pages != 0).any(-1).nonzero().tolist()
+    assert written == [[1, 2], [1, 3], [4, 15], [5, 0]]        # positions 18 and 19, 31 and 32
