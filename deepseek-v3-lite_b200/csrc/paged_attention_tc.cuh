@@ -79,7 +79,7 @@ inline bool paged_plan(int N, int R, int D, PagedPlan& p) {
   p.nch = (D + 63) / 64;
   p.tail = D > 128 * p.LP ? 1 : 0;
   p.tails = p.tail ? 2 : 0;
-  const int q = p.nch * N * 128, P = (N + 63) / 64 * chunk, misc = 28 * N + 520;
+  const int q = p.nch * N * 128, P = (N + 63) / 64 * chunk, misc = 28 * N + 448 + pa_threads(N) / 4;
   // a second P buffer where the ring still holds two key tiles with it
   for (p.pbufs = 2;; --p.pbufs) {
     const int fit = (kPaSmem - q - p.pbufs * P - p.tails * chunk - misc) / (2 * chunk);
@@ -297,31 +297,35 @@ struct PagedStart {
   int local;                  // its index within sequence b
   int b, rt, tile, found;
   int gap;                    // the offsets do not cover every token once
+  int excess;                 // more key tiles than 32 bits count
 };
 
 template <int N>
-__device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, PagedStart* out, int* scan,
+__device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, PagedStart* out, int2* scan,
                                            unsigned int* status) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int THREADS = pa_threads(N), NW = THREADS / 32;
-  if (tid == 0) out->gap = 0;
+  if (tid == 0) out->gap = out->excess = 0;
   // round 0 adds up all sequences; round 1 finds the one that holds the share's
   // first tile (a batch of up to THREADS sequences is still in registers)
   int target = 0, t = 0;
   PagedSeq s;
   s.tiles = 0;
   for (int round = 0; round < 2; ++round) {
-    int base = 0;
+    int base = 0, thousands = 0;             // key tiles, and by 1,024 rounded up per sequence
     for (int b0 = 0; b0 < r.B; b0 += THREADS) {
       const int b = b0 + tid;
       bool gap = false;
+      int more = 0;
       if (round == 0 || r.B > THREADS) {
         s.tiles = 0;
         t = 0;
         if (b < r.B) {
           s = paged_seq<N>(r, b, H, total);
-          t = (int)paged_tiles_before<N>(s, s.tiles, H);
+          const long long tiles = paged_tiles_before<N>(s, s.tiles, H);
+          t = (int)tiles;
           if (round == 0) {
+            more = (int)min((tiles + 1023) >> 10, 1ll << 21);
             const int c0 = __ldg(r.cu + b), c1 = __ldg(r.cu + b + 1);
             gap = c1 > total || c1 < c0 || (b == 0 && c0 != 0) || (b == r.B - 1 && c1 != total);
             if (blockIdx.x == 0 && (gap || __ldg(r.lens + b) > r.cols * r.page)) record_error(status, DSV3_ERR_BOUNDS);
@@ -334,15 +338,17 @@ __device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, Pa
         const int v = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += v;
       }
-      if (lane == 31) scan[warp] = inc;
+      more = __reduce_add_sync(0xffffffffu, more);
+      if (lane == 31) scan[warp] = make_int2(inc, more);
       __syncthreads();
       if (gap) out->gap = 1;
       int before = base, all = base;
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        const int v = scan[w];
-        if (w < warp) before += v;
-        all += v;
+        const int2 v = scan[w];
+        if (w < warp) before += v.x;
+        all += v.x;
+        thousands = min(thousands + v.y, 1 << 21);
       }
       if (round == 1 && t > 0 && before + inc - t <= target && target < before + inc) {
         out->b = b;
@@ -356,6 +362,13 @@ __device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, Pa
       __syncthreads();
     }
     if (round == 0) {
+      if (thousands >= (1 << 21) - 1024) {     // reported, and nothing is computed
+        if (tid == 0) {
+          out->excess = 1;
+          if (blockIdx.x == 0) record_error(status, DSV3_ERR_BOUNDS);
+        }
+        base = 0;
+      }
       int share = (base + gridDim.x - 1) / gridDim.x;
       target = share * blockIdx.x;
       if (tid == 0) {
@@ -392,16 +405,16 @@ __device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, Pa
   }
 }
 
-// Zeroes the result of the tokens that no sequence holds; the whole CTA, a token
-// per CTA in turn.  Only for offsets that are reported as wrong.
-__device__ __forceinline__ void paged_clear_gaps(const Ragged& r, int total, size_t row_bytes, uint8_t* out) {
+// Zeroes the result of the tokens that no sequence holds, or of all; the whole CTA,
+// a token per CTA in turn.  Only for metadata that are reported as wrong.
+__device__ __forceinline__ void paged_clear(const Ragged& r, bool all, int total, size_t row_bytes, uint8_t* out) {
 #pragma unroll 1
   for (int t = blockIdx.x; t < total; t += gridDim.x) {
     bool held = false;
 #pragma unroll 1
     for (int b = threadIdx.x; b < r.B; b += blockDim.x) {
       const int c0 = __ldg(r.cu + b), c1 = __ldg(r.cu + b + 1);
-      held |= c0 >= 0 && c1 <= total && c0 <= t && t < c1;
+      held |= !all && c0 >= 0 && c1 <= total && c0 <= t && t < c1;
     }
     if (__syncthreads_or(held)) continue;
 #pragma unroll 1
@@ -568,7 +581,7 @@ __global__ void __launch_bounds__(pa_threads(N), 1) paged_attention_tc_kernel(
   uint64_t* s_free = o_free + 1;      // [2]
   uint64_t* drain = s_free + 2;       // [2]
   PagedStart* start = reinterpret_cast<PagedStart*>(drain + 2);
-  int* scan = reinterpret_cast<int*>(start + 1);             // [threads / 32]
+  int2* scan = reinterpret_cast<int2*>(start + 1);           // [threads / 32]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(scan + pa_threads(N) / 32);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -609,7 +622,8 @@ __global__ void __launch_bounds__(pa_threads(N), 1) paged_attention_tc_kernel(
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (start->gap) paged_clear_gaps(rg, total, (size_t)H * R * 2, reinterpret_cast<uint8_t*>(out));
+  if (start->gap | start->excess)
+    paged_clear(rg, start->excess, total, (size_t)H * R * 2, reinterpret_cast<uint8_t*>(out));
   const uint32_t tmem = warp_uniform(*tmem_slot);
   const int count = warp_uniform(start->count), b_0 = warp_uniform(start->b), rt_0 = warp_uniform(start->rt),
             tile_0 = warp_uniform(start->tile);

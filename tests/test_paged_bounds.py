@@ -236,3 +236,17 @@ def test_append_skips_tokens_of_no_sequence(rank, rope, reported):
     reported()
     written = (pages != 0).any(-1).nonzero().tolist()
     assert written == [[1, 2], [1, 3], [4, 15], [5, 0]]        # positions 18 and 19, 31 and 32
+
+
+@pytest.mark.gpu
+def test_attention_reports_more_key_tiles_than_it_counts(reported):
+    """2^20 rows over 2^24 cached ones (of one page): not computed, zeros and a report."""
+    from ops.paged import paged_latent_attention
+    q = torch.ones(256, 4096, 24, device="cuda", dtype=torch.bfloat16)
+    pages = torch.ones(1, 256, 24, device="cuda", dtype=torch.bfloat16)
+    table = torch.zeros(1, 1 << 16, dtype=torch.int32, device="cuda")
+    out = paged_latent_attention(q, pages, table, _i32([0, 256], "cuda"), _i32([1 << 24], "cuda"), 16, 0.1)
+    reported()
+    assert (out == 0).all()
+    out = paged_latent_attention(q[:2], pages, table, _i32([0, 2], "cuda"), _i32([1 << 16], "cuda"), 16, 0.1)
+    assert (out == 1).all()
