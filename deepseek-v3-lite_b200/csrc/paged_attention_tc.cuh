@@ -61,6 +61,8 @@ constexpr int KT = 64;                       // key tile
 constexpr int kPaMaxSlots = 16;
 constexpr int kPaSmem = 232448;              // shared memory of a CTA, at most
 constexpr float kPaUnset = -1e30f;           // reference of a row that has seen no key
+constexpr float kPaNever = 1e30f;            // of one that sees none, or lies past the sequence's rows: the tile
+                                             // holds the next sequence's queries there, whose scores have no vote
 constexpr float kPaLead = 12.f;              // first reference above the first key's score (log2)
 
 struct PagedPlan {
@@ -849,11 +851,12 @@ __global__ void __launch_bounds__(pa_threads(N), 1) paged_attention_tc_kernel(
           if (key == 0) {
 #pragma unroll
             for (int c = 0; c < NC; c += 4) {
+              const int4 k4 = lim4[c / 4];
               float4 m4;
-              m4.x = fmaxf(fmaf(__uint_as_float(sr[c]), scale_log2, kPaLead), kPaUnset);
-              m4.y = fmaxf(fmaf(__uint_as_float(sr[c + 1]), scale_log2, kPaLead), kPaUnset);
-              m4.z = fmaxf(fmaf(__uint_as_float(sr[c + 2]), scale_log2, kPaLead), kPaUnset);
-              m4.w = fmaxf(fmaf(__uint_as_float(sr[c + 3]), scale_log2, kPaLead), kPaUnset);
+              m4.x = k4.x > 0 ? fmaxf(fmaf(__uint_as_float(sr[c]), scale_log2, kPaLead), kPaUnset) : kPaNever;
+              m4.y = k4.y > 0 ? fmaxf(fmaf(__uint_as_float(sr[c + 1]), scale_log2, kPaLead), kPaUnset) : kPaNever;
+              m4.z = k4.z > 0 ? fmaxf(fmaf(__uint_as_float(sr[c + 2]), scale_log2, kPaLead), kPaUnset) : kPaNever;
+              m4.w = k4.w > 0 ? fmaxf(fmaf(__uint_as_float(sr[c + 3]), scale_log2, kPaLead), kPaUnset) : kPaNever;
               mref4[c / 4] = m4;
             }
           }

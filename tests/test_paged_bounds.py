@@ -250,3 +250,25 @@ def test_attention_reports_more_key_tiles_than_it_counts(reported):
     assert (out == 0).all()
     out = paged_latent_attention(q[:2], pages, table, _i32([0, 2], "cuda"), _i32([1 << 16], "cuda"), 16, 0.1)
     assert (out == 1).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,rank,new", [(12, 192, 1), (5, 64, 1), (20, 512, 1), (12, 192, 7), (16, 512, 5)])
+def test_attention_of_a_sequence_ignores_its_neighbours(heads, rank, new):
+    """A row tile's spare rows hold the next sequence's queries; peaked ones there change no bit of the result."""
+    from ops._ext import check_status
+    from ops.paged import paged_latent_attention
+    g = torch.Generator(device="cuda").manual_seed(heads)
+    batch, cols, page = 30, 40, 32
+    width = rank + 24
+    pages = torch.randn(batch * cols, page, width, device="cuda", generator=g).bfloat16()
+    table = torch.randperm(batch * cols, device="cuda", generator=g).int().view(batch, cols)
+    lens = torch.randint(new, cols * page, (batch,), device="cuda", generator=g).int()
+    cu = _i32([new * b for b in range(batch + 1)], "cuda")
+    q = torch.randn(batch, new, heads, width, device="cuda", generator=g)
+    peaked = q.clone()
+    peaked[1::2] *= 30.0
+    want, got = [paged_latent_attention(x.bfloat16().flatten(0, 1), pages, table, cu, lens, rank, width ** -0.5)
+                 for x in (q, peaked)]
+    check_status()
+    assert torch.equal(got.view(batch, new, heads, rank)[::2], want.view(batch, new, heads, rank)[::2])
