@@ -7,6 +7,7 @@
 #include <torch/extension.h>
 
 #include <mutex>
+#include <string>
 
 namespace dsv3 {
 
@@ -48,7 +49,7 @@ inline CUtensorMap make_map(const void* ptr, int rank, const uint64_t* dims, con
   CUresult r = encode_fn()(&m, dtype, rank, const_cast<void*>(ptr), d, s, b, e,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code ", int(r));
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code ", std::to_string(int(r)));
   return m;
 }
 

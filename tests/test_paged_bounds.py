@@ -272,3 +272,13 @@ def test_attention_of_a_sequence_ignores_its_neighbours(heads, rank, new):
                  for x in (q, peaked)]
     check_status()
     assert torch.equal(got.view(batch, new, heads, rank)[::2], want.view(batch, new, heads, rank)[::2])
+
+
+@pytest.mark.gpu
+def test_a_layout_that_tma_refuses_raises():
+    """A page stride of 2^40 bytes (of a pool of one page): an exception with the driver's code, not a crash."""
+    from ops.paged import paged_latent_attention
+    pages = torch.zeros(64 * 80, device="cuda", dtype=torch.bfloat16).as_strided((1, 64, 80), (1 << 39, 80, 1))
+    q = torch.zeros(1, 4, 80, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="cuTensorMapEncodeTiled failed with code [0-9]+"):
+        paged_latent_attention(q, pages, _i32([[0]], "cuda"), _i32([0, 1], "cuda"), _i32([5], "cuda"), 64, 0.1)
