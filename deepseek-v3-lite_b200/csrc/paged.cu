@@ -288,9 +288,11 @@ at::Tensor paged_latent_attention(const at::Tensor& q, const at::Tensor& pages, 
   TORCH_CHECK(rg.B > 0, op, ": tokens without a sequence");
   const at::cuda::CUDAGuard guard(pages.device());
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  // Row tile: 16 and 32 where a sequence has that many rows on average (a
-  // decode step), else 64, or 128 where the output columns of a 128-row tile
-  // fit in TMEM and the sequences fill it.
+  // Row tile, from the rows per sequence on average: 16 up to 16; 32 up to 32 where
+  // every sequence has one token (24 heads of R 192 over 64 x 2,048 rows 26.7 us
+  // against 30.4 with 64; 32 heads of R 512 45.4 against 50.6), while a ragged batch
+  // of the same average may hold chunks, which want 64; then 64, or 128 where the
+  // output columns of a 128-row tile fit in TMEM and the sequences fill it.
   const int64_t rows = (T * H + rg.B - 1) / rg.B;
   const int N = rows <= 16 ? 16 : rows <= 32 && T == rg.B ? 32 : rows <= 64 || R > 256 ? 64 : 128;
   PagedPlan pl;
