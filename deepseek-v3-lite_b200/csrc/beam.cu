@@ -622,11 +622,13 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> beam_select(const at:
 at::Tensor beam_reorder(at::Tensor& pages, const at::Tensor& table, const at::Tensor& parents,
                         const at::Tensor& lens) {
   const char* op = "beam_reorder";
-  TORCH_CHECK(pages.is_cuda() && pages.dim() == 4 && pages.stride(3) == 1 && pages.stride(2) == pages.size(3), op,
+  TORCH_CHECK(pages.is_cuda() && pages.dim() == 4 &&
+                  (pages.numel() == 0 || (pages.stride(3) == 1 && pages.stride(2) == pages.size(3))), op,
               ": pages must be a CUDA tensor [layers, pool, page, width] with contiguous pages");
   const int64_t es = pages.element_size(), width = pages.size(3), page = pages.size(2);
-  TORCH_CHECK(width * es % 16 == 0 && pages.stride(0) * es % 16 == 0 && pages.stride(1) * es % 16 == 0 &&
-                  reinterpret_cast<uintptr_t>(pages.data_ptr()) % 16 == 0 && page >= 1,
+  TORCH_CHECK(pages.numel() == 0 ||
+                  (width * es % 16 == 0 && pages.stride(0) * es % 16 == 0 && pages.stride(1) * es % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(pages.data_ptr()) % 16 == 0),
               op, ": page rows must be 16-byte aligned");
   TORCH_CHECK(parents.dim() == 2 && parents.scalar_type() == at::kInt && parents.is_contiguous() &&
                   parents.device() == pages.device(),
@@ -639,14 +641,19 @@ at::Tensor beam_reorder(at::Tensor& pages, const at::Tensor& table, const at::Te
   TORCH_CHECK(lens.dim() == 1 && lens.scalar_type() == at::kInt && lens.is_contiguous() && lens.size(0) == B &&
                   lens.device() == pages.device(),
               op, ": seq_lens must be a contiguous int32 tensor [B]");
+  TORCH_CHECK(page >= 1, op, ": an empty page");
   TORCH_CHECK(B <= 65535 && pages.size(0) <= 65535 && pages.size(1) < (1ll << 31), op, ": too many groups or layers");
   const at::cuda::CUDAGuard guard(pages.device());
   auto out = at::Tensor(at::detail::empty_cuda({B * K, table.size(1)}, at::kInt, pages.device(), c10::nullopt));
   if (B == 0 || table.size(1) == 0) return out;
   const int row16 = (int)(width * es / 16);
-  const int parts = (int)((page * row16 + kCopyThreads * kCopyVecs - 1) / (kCopyThreads * kCopyVecs));
-  const int splits = (int)std::max<int64_t>(1, K / 2);   // about K / e copies per group when parents are random
-  const dim3 grid(parts * splits + 1, (unsigned)std::max<int64_t>(1, pages.size(0)), (unsigned)B);
+  const int64_t layers = pages.numel() == 0 ? 0 : pages.size(0);
+  const int64_t vecs = page * row16, per = kCopyThreads * kCopyVecs;
+  const int parts = (int)std::max<int64_t>(1, (vecs + per - 1) / per);
+  // about K / e copies per group when parents are random; none without layers, where
+  // the one CTA of a group writes its table
+  const int splits = layers == 0 ? 0 : (int)std::max<int64_t>(1, K / 2);
+  const dim3 grid(parts * splits + 1, (unsigned)std::max<int64_t>(1, layers), (unsigned)B);
   beam_reorder_kernel<<<grid, kCopyThreads, 0, at::cuda::getCurrentCUDAStream()>>>(
       reinterpret_cast<uint4*>(pages.data_ptr()), pages.stride(0) * es / 16, pages.stride(1) * es / 16, row16,
       (int)page, (int)pages.size(1), table.data_ptr<int>(), table.stride(0), (int)table.size(1),

@@ -282,3 +282,14 @@ def test_a_layout_that_tma_refuses_raises():
     q = torch.zeros(1, 4, 80, device="cuda", dtype=torch.bfloat16)
     with pytest.raises(RuntimeError, match="cuTensorMapEncodeTiled failed with code [0-9]+"):
         paged_latent_attention(q, pages, _i32([[0]], "cuda"), _i32([0, 1], "cuda"), _i32([5], "cuda"), 64, 0.1)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_reorder_of_a_table_alone(device):
+    """Pages without a layer, or without a column: the new table, and no copy."""
+    from ops.beam import beam_reorder
+    table = torch.arange(12, dtype=torch.int32, device=device).view(4, 3)
+    for shape in ((0, 12, 16, 32), (2, 12, 16, 0)):
+        pages = torch.zeros(shape, device=device, dtype=torch.bfloat16)
+        out = beam_reorder(pages, table, _i32([[1, 1, 2, 1]], device), _i32([21], device))
+        assert out.tolist() == [[3, 4, 2], [3, 1, 5], [6, 7, 8], [3, 10, 11]]
