@@ -12,8 +12,13 @@
 //   O^T [R x N rows]      += V^T [R x KT keys] . P^T            (the same K, read MN-major)
 //
 // KT is 64: with R 512 and N 64 the shared memory then holds two key tiles (128
-// rows left no room for a second; 441 us against 361 us for 4 x 512 new tokens),
-// and an MMA of 64 keys and 64 rows takes 32 cycles against 48 of 128 keys.
+// rows left no room for a second; 441 us against 361 us for 4 x 512 new tokens when
+// it was chosen), and an MMA of 64 keys and 64 rows takes 32 cycles against 48 of
+// 128 keys.
+//
+// P is bf16 because an MMA takes one type for both of its operands and the cache is
+// bf16.  Each weight is then off by 2^-9 at most, as the result is by its own
+// rounding; all else (scores, references, sums, O, partials) is fp32.
 //
 // The cache row [latent | rotated key] is read as 64-column chunks [KT x 64]
 // with a 128-byte swizzle; chunk pairs 0 .. LP-1 cover the latent (LP =
@@ -44,13 +49,14 @@
 // bounded; after one ran out the softmax warps go on without waiting, so that
 // they meet at their barriers, and the others stop.
 //
-// Measured (R 512, 16 heads, pages of 64): 64 requests with 512 to 4,096 rows, one
-// token each, 39 us without the merge (169 MB, floor 26 us); two of 100,000 rows
-// 60 us (floor 42 us); 4 x 512 new tokens on 3,000 to 4,096 rows 361 us, 650
-// TFLOP/s: both products read their operands from shared memory at its full rate,
-// and TMA writes the key tiles into it as well (2,600 of the 3,300 cycles of a
-// tile).  R 192, 16 ragged chunks of up to 509 tokens: 78 us, bound by the softmax
-// and by the turn from one row tile to the next.
+// Measured on the device, without the merge (R 512, 16 heads, pages of 64): 64
+// requests with 512 to 4,096 rows, one token each, 40 us (169 MB, floor 26 us; 4.1
+// TB/s with a cold L2); two of 100,000 rows 60 us (floor 42 us); 4 x 512 new tokens
+// on 3,000 to 4,096 rows 365 us with the merge, 630 TFLOP/s: tensor pipe active in
+// 44% of the cycles, its operand path in 48%, which is S^T with 64 keys on the M side
+// and 64 rows on the N side of both.  R 192, 16 ragged chunks of up to 509 tokens: 79
+// us, tensor pipe 28%, bound by the softmax and by the turn from one row tile to the
+// next.
 
 // Softmax warpgroups of a row tile, each with its share of the rows: two for few
 // rows; four for 64 and 128, where the softmax of a tile takes longer than its MMAs
@@ -126,7 +132,7 @@ __device__ __forceinline__ long long floor_sum(T n, T m, T a, T b) {
 
 // One sequence as the scheduler sees it.
 struct PagedSeq {
-  int tok0, n, len;           // first token, new tokens, cached length
+  int tok0, end, n, len;      // first token, the one after the last, new tokens, cached length
   int rows, tiles;            // (token, head) rows, row tiles of N
 };
 
@@ -135,6 +141,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const Ragged& r, int b, int H, int
   PagedSeq s;
   const int c0 = __ldg(r.cu + b), c1 = __ldg(r.cu + b + 1);
   s.tok0 = c0;
+  s.end = c1;
   s.n = (c0 >= 0 && c1 <= total && c1 > c0) ? c1 - c0 : 0;
   s.len = min(max(__ldg(r.lens + b), 0), r.cols * r.page);
   s.rows = s.n * H;
@@ -328,8 +335,7 @@ __device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, Pa
           t = (int)tiles;
           if (round == 0) {
             more = (int)min((tiles + 1023) >> 10, 1ll << 21);
-            const int c0 = __ldg(r.cu + b), c1 = __ldg(r.cu + b + 1);
-            gap = c1 > total || c1 < c0 || (b == 0 && c0 != 0) || (b == r.B - 1 && c1 != total);
+            gap = s.end > total || s.end < s.tok0 || (b == 0 && s.tok0 != 0) || (b == r.B - 1 && s.end != total);
             if (blockIdx.x == 0 && (gap || __ldg(r.lens + b) > r.cols * r.page)) record_error(status, DSV3_ERR_BOUNDS);
           }
         }
@@ -350,8 +356,9 @@ __device__ __forceinline__ void paged_find(const Ragged& r, int H, int total, Pa
         const int2 v = scan[w];
         if (w < warp) before += v.x;
         all += v.x;
-        thousands = min(thousands + v.y, 1 << 21);
+        thousands += v.y;                      // (at most 19 warps of 32 x 2^21)
       }
+      thousands = min(thousands, 1 << 21);
       if (round == 1 && t > 0 && before + inc - t <= target && target < before + inc) {
         out->b = b;
         out->local = target - (before + inc - t);
