@@ -144,7 +144,8 @@ __device__ __forceinline__ void cta_rank(int k, uint32_t threshold, bool any, in
 // nothing above the last of them costs one barrier.  The logits of the next
 // segment are on their way while this one is looked at.  A thread's elements go
 // by their index in the row, never by its address, so that sums and scores are
-// the same wherever a row lies.  Bound by reading the logits.
+// the same wherever a row lies.  32 x 8 rows of 102,400 fp32 take 34 us (16 at the
+// copy rate): the ranking of a part's first segments bounds it, not the reads.
 template <typename T, int THREADS, int PER, bool ALIGNED>
 __global__ void __launch_bounds__(THREADS, 3) beam_scan_kernel(const T* __restrict__ logits, long ldb, long ldk,
                                                                             int units, int nseg, int chunk, int runs,

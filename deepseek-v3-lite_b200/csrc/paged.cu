@@ -116,8 +116,8 @@ __device__ __forceinline__ void load8(const bf16* p, float (&v)[8]) {
 // The same where rows are 16-byte aligned, R and dr multiples of 8 and R + dr at
 // most 768: a lane takes up to three groups of 8 columns, read once, on their way
 // while the token's sequence and page are looked up.  Bound by that latency for a
-// decode step, by the bytes for a prompt (8,000 rows of 576: 3.0 us at the copy
-// rate).
+// decode step (64 rows: 3.1 us on the device), by it and the bytes for a prompt
+// (8,300 rows of 576: 6.6 us, of which the bytes take 3.0 at the copy rate).
 template <typename T>
 __global__ void __launch_bounds__(128) latent_append_vec_kernel(const T* __restrict__ x, long ldx, int total, int R,
                                                                 int dr, float eps, const float* __restrict__ w,
@@ -288,11 +288,13 @@ at::Tensor paged_latent_attention(const at::Tensor& q, const at::Tensor& pages, 
   TORCH_CHECK(rg.B > 0, op, ": tokens without a sequence");
   const at::cuda::CUDAGuard guard(pages.device());
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  // Row tile, from the rows per sequence on average: 16 up to 16; 32 up to 32 where
-  // every sequence has one token (24 heads of R 192 over 64 x 2,048 rows 26.7 us
-  // against 30.4 with 64; 32 heads of R 512 45.4 against 50.6), while a ragged batch
-  // of the same average may hold chunks, which want 64; then 64, or 128 where the
-  // output columns of a 128-row tile fit in TMEM and the sequences fill it.
+  // Row tile, from the rows per sequence on average: 16 up to 16 (12 heads of R 192
+  // over 64 x 2,048 rows 24.6 us against 26.7 with 32); 32 up to 32 where every
+  // sequence has one token (24 heads 26.7 against 30.4 with 64; of R 512, 32 heads,
+  // 45.4 against 50.6), while a ragged batch of the same average may hold chunks,
+  // which want 64; 64 up to 64 (32 x 5 tokens of 12 heads 26.7 against 28.7 with
+  // 128); then 128 (8 x 256 tokens 77.5 against 98.4 with 64) where the output
+  // columns of 128 rows fit in TMEM.
   const int64_t rows = (T * H + rg.B - 1) / rg.B;
   const int N = rows <= 16 ? 16 : rows <= 32 && T == rg.B ? 32 : rows <= 64 || R > 256 ? 64 : 128;
   PagedPlan pl;

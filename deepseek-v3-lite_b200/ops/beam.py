@@ -1,7 +1,8 @@
 """Beam search: choosing the next beams and reordering their paged cache.
 
 CUDA tensors run the kernels of ``csrc/beam.cu``, CPU tensors the formulas
-below (also the numerics oracle of the kernel tests).
+below (also the numerics oracle of the kernel tests).  Neither has a backward
+pass; on CUDA results are detached.
 """
 from __future__ import annotations
 
