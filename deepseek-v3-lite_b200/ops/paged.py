@@ -23,7 +23,7 @@ two from 8 to 256; R is a multiple of 8 up to 512 and dr one up to 64.
 CUDA tensors run the kernels of ``csrc/paged.cu``, CPU tensors the formulas
 below.  On CUDA a page or position out of range, or a token that the offsets
 leave out, is skipped and reported by ``ops._ext.check_status``; on the CPU it
-raises ``IndexError``.
+raises ``IndexError`` (the attention alone gives a token left out zeros).
 
 These operators serve: they have no backward pass.  On CUDA their results are
 detached, whether gradients are enabled or not (``models.mla`` trains).
@@ -106,7 +106,7 @@ def paged_latent_attention(q: torch.Tensor, pages: torch.Tensor, block_table: to
     followed by its rotated part (dr).  Row ``t`` sees the cached rows up to its
     own position; the result ``[T, H, R]`` is the weighted sum of their latents.
     A token that sees no row (its position is negative) or that no sequence holds
-    (reported) gets zeros.  Rows at and
+    (reported on CUDA) gets zeros.  Rows at and
     past ``seq_lens`` may hold anything; those before it have to be finite, also
     for earlier tokens that do not see them (their weight there is zero, and zero
     times infinity is not).  ``scale`` is positive; ``q`` is copied if it is not
